@@ -443,6 +443,52 @@ int lancet_softmax_xent_fwd(const void* logits, long long ld, const long long* t
 int lancet_softmax_xent_bwd(const void* logits, long long ld, const long long* target, int rows, int vocab, int cols, int dtype,
                             const float* lse_rows, const float* grad_out, float scale, void* dlogits, long long ldd,
                             lancet_stream_t stream);
+/* Losses of the language-model head from its hidden rows, the logits never in memory as a whole (the pair of operators above takes logits;
+ * the reference's models end in a dense layer + log_softmax + nll_loss, models/benchmark/raf/raf_bencher.py:84).
+ * hidden [rows][ldh], weight [>= vocab rows][ldw] (the weight's rows start on 16-byte boundaries: ldw % 8 == 0), both bfloat16 or both
+ * float16; z = hidden * weight[:vocab]^T.
+ *   lse_rows[r] = log sum_j exp(z[r][j] / T), T = 1 for the cross entropy
+ *   loss_rows[r] = lse_rows[r] - z[r][target[r]]
+ *   loss_rows[r] = T^2 sum_i q_i (log q_i - z[r][idx_i] / T + lse_rows[r]), q = softmax(v / T) over the row's teacher entries that count
+ * target [rows] int64, negative or >= vocab = row ignored.  Teacher: top_values [rows][k] (float32, float16 or bfloat16) and
+ * top_indices [rows][k] int64, k <= 512; an index that names no class does not count, a class named twice gets both weights, a row whose
+ * counting values are none or all -inf is ignored.  Ignored rows: loss and lse 0, gradient row 0, and their hidden rows are not used (they
+ * may hold anything).  0.001 <= temperature <= 1000.
+ * pos [rows + 1] int32: packed index of every row that takes part or -1, then their number; diff [rows][k] float32: student minus teacher
+ * probability at the teacher's classes; the backward calls take both.  mean = sum(loss_rows) * inv_live, inv_live = 1 / max(live rows, 1)
+ * (float32 scalars on the device).
+ * ws: lancet_linear_loss_*_workspace_bytes bytes (k = 0 for the cross entropy), 256-byte aligned, used by this call only.  status: int32 on
+ * the device, as for the grouped GEMM. */
+size_t lancet_linear_loss_fwd_workspace_bytes(int rows, int vocab, int width, int k);
+size_t lancet_linear_loss_bwd_workspace_bytes(int rows, int vocab, int width);
+int lancet_linear_xent_fwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, int rows, int vocab,
+                           int width, int dtype, float* loss_rows, float* lse_rows, int32_t* pos, float* mean, float* inv_live, void* ws,
+                           size_t ws_bytes, int32_t* status, lancet_stream_t stream);
+int lancet_linear_distill_fwd(const void* hidden, long long ldh, const void* weight, long long ldw, const void* top_values, int values_dtype,
+                              const long long* top_indices, int k, float temperature, int rows, int vocab, int width, int dtype,
+                              float* loss_rows, float* lse_rows, float* diff, int32_t* pos, float* mean, float* inv_live, void* ws,
+                              size_t ws_bytes, int32_t* status, lancet_stream_t stream);
+/* Gradients of sum(loss_rows) * (*grad_out) * (*inv_live) * scale (null pointers count as 1): dhidden [rows][width], dweight
+ * [weight_rows][width] (rows from vocab on are zero), in the operands' type, rounded once; either may be null and is then not computed.
+ * dz = d loss / d z is formed a piece of the vocabulary at a time, in 16 bits (workspace: 2 bytes x rows x classes of a piece). */
+int lancet_linear_xent_bwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target,
+                           const float* loss_rows, const float* lse_rows, const int32_t* pos, int rows, int vocab, int weight_rows, int width,
+                           int dtype, const float* grad_out, const float* inv_live, float scale, void* dhidden, void* dweight, void* ws,
+                           size_t ws_bytes, int32_t* status, lancet_stream_t stream);
+int lancet_linear_distill_bwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* top_indices,
+                              const float* diff, int k, float temperature, const float* lse_rows, const int32_t* pos, int rows, int vocab,
+                              int weight_rows, int width, int dtype, const float* grad_out, const float* inv_live, float scale, void* dhidden,
+                              void* dweight, void* ws, size_t ws_bytes, int32_t* status, lancet_stream_t stream);
+/* The distillation loss on given logits [rows][ld] (float32, float16 or bfloat16; columns from vocab on are padding and never read), the
+ * soft-target counterpart of lancet_softmax_xent_*; teacher, ignored rows, mean and inv_live as above.  class_weights [rows][k] float32 (the
+ * teacher's probability of each entry's class) and live_rows [rows] int32 are kept for the backward call, which writes the gradient in the
+ * logits' type: zero in padded columns and ignored rows. */
+int lancet_distill_fwd(const void* logits, long long ld, const void* top_values, int values_dtype, const long long* top_indices, int k,
+                       float temperature, int rows, int vocab, int dtype, float* loss_rows, float* lse_rows, float* class_weights,
+                       int32_t* live_rows, float* mean, float* inv_live, lancet_stream_t stream);
+int lancet_distill_bwd(const void* logits, long long ld, const long long* top_indices, const float* class_weights, const int32_t* live_rows,
+                       int k, float temperature, int rows, int vocab, int cols, int dtype, const float* lse_rows, const float* grad_out,
+                       const float* inv_live, float scale, void* dlogits, long long ldd, lancet_stream_t stream);
 /* Bias gradient of an expert layer: db[e][:] = sum over the groups of expert e and their live rows of
  * dY[g][r][:]  (dY [groups][C][N], db [LE][N]); the reference gets it from the autodiff of nn.Linear's
  * bias add (a `sum` over rows).  ws: lancet_grouped_bias_grad_workspace_bytes(LE, N) bytes. */

@@ -164,6 +164,25 @@ SIGNATURES = {
     "lancet_softmax_xent_fwd": (c_int, [c_void_p, ctypes.c_longlong, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "lancet_softmax_xent_bwd": (c_int, [c_void_p, ctypes.c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
                                         ctypes.c_float, c_void_p, ctypes.c_longlong, c_void_p]),
+    "lancet_linear_loss_fwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "lancet_linear_loss_bwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "lancet_linear_xent_fwd": (c_int, [c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_longlong, c_void_p, c_int, c_int,
+                                       c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                                       c_void_p, c_void_p]),
+    "lancet_linear_distill_fwd": (c_int, [c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_longlong, c_void_p, c_int,
+                                          c_void_p, c_int, c_float, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                                          c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "lancet_linear_xent_bwd": (c_int, [c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_longlong, c_void_p, c_void_p,
+                                       c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_float,
+                                       c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "lancet_linear_distill_bwd": (c_int, [c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_longlong, c_void_p, c_void_p,
+                                          c_int, c_float, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p,
+                                          c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "lancet_distill_fwd": (c_int, [c_void_p, ctypes.c_longlong, c_void_p, c_int, c_void_p, c_int, c_float, c_int, c_int,
+                                   c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "lancet_distill_bwd": (c_int, [c_void_p, ctypes.c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_float, c_int, c_int,
+                                   c_int, c_int, c_void_p, c_void_p, c_void_p, c_float, c_void_p, ctypes.c_longlong,
+                                   c_void_p]),
     "lancet_peer_copy": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "lancet_lans_dev_step": (c_int, [c_void_p, c_size_t, c_int, ctypes.POINTER(c_i64), ctypes.POINTER(c_void_p),
                                      ctypes.POINTER(c_void_p), ctypes.POINTER(c_void_p), ctypes.POINTER(c_void_p), c_int,

@@ -3,6 +3,7 @@ builders wrap MOELayerImpl the same way, models/benchmark/pytorch/utils.py:576-6
 library's forward and backward.  torch is the host framework here; every MoE kernel is the library's."""
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from .layer import MoELayer
@@ -288,6 +289,89 @@ def softmax_cross_entropy(logits, target, vocab=None):
     language-model head of the reference's benchmark models (log_softmax + nll_loss, models/benchmark/raf/raf_bencher.py:84)
     without float32 copies of the [tokens, vocabulary] matrix."""
     return _SoftmaxCrossEntropy.apply(logits, target, logits.shape[1] if vocab is None else vocab)
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, target, vocab):
+        loss_rows, lse, mean, inv_live, pos = ops.linear_xent_fwd(hidden, weight, target, vocab)
+        ctx.save_for_backward(hidden, weight, target, loss_rows, lse, pos, inv_live)
+        ctx.vocab = vocab
+        return mean
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gout):
+        hidden, weight, target, loss_rows, lse, pos, inv_live = ctx.saved_tensors
+        dh, dw = ops.linear_xent_bwd(hidden, weight, target, loss_rows, lse, pos, ctx.vocab, gout, inv_live,
+                                     need_hidden=ctx.needs_input_grad[0], need_weight=ctx.needs_input_grad[1])
+        return dh, dw, None, None
+
+
+class _LinearDistillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, top_values, top_indices, temperature, vocab):
+        _, lse, mean, inv_live, pos, diff = ops.linear_distill_fwd(hidden, weight, top_values, top_indices, temperature, vocab)
+        ctx.save_for_backward(hidden, weight, top_indices, lse, pos, diff, inv_live)
+        ctx.temperature, ctx.vocab = temperature, vocab
+        return mean
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gout):
+        hidden, weight, top_indices, lse, pos, diff, inv_live = ctx.saved_tensors
+        dh, dw = ops.linear_distill_bwd(hidden, weight, top_indices, diff, lse, pos, ctx.temperature, ctx.vocab, gout, inv_live,
+                                        need_hidden=ctx.needs_input_grad[0], need_weight=ctx.needs_input_grad[1])
+        return dh, dw, None, None, None, None
+
+
+class _Distillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_values, top_indices, temperature, vocab):
+        _, lse, mean, inv_live, live, weights = ops.distill_fwd(logits, top_values, top_indices, temperature, vocab)
+        ctx.save_for_backward(logits, top_indices, weights, live, lse, inv_live)
+        ctx.temperature, ctx.vocab = temperature, vocab
+        return mean
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gout):
+        logits, top_indices, weights, live, lse, inv_live = ctx.saved_tensors
+        return ops.distill_bwd(logits, top_indices, weights, live, lse, ctx.temperature, ctx.vocab, gout, inv_live), None, None, None, None
+
+
+def _head_inputs(hidden, weight):
+    """Rows of the head as F.linear would see them: any leading axes, the autocast type inside an autocast region."""
+    hidden = hidden.reshape(-1, hidden.shape[-1])
+    if hidden.is_cuda and torch.is_autocast_enabled("cuda"):
+        dt = torch.get_autocast_dtype("cuda")
+        hidden, weight = hidden.to(dt), weight.to(dt)
+    return hidden, weight
+
+
+def linear_cross_entropy(hidden, weight, target, vocab=None):
+    """Mean cross entropy of the language-model head from its hidden rows, equal to
+    `softmax_cross_entropy(F.linear(hidden, weight), target, vocab)` without the [rows, classes] logits and their gradient in memory.
+    hidden [..., width] and weight [classes, width] bfloat16 or float16 of one type (inside an autocast region: cast to its type), target
+    [...] int64 (negative or >= vocab = ignored), weight rows from `vocab` on are padding.  The sums are float32; the gradient of the logits
+    passes between the products in the operands' type, as it does between a loss and F.linear."""
+    hidden, weight = _head_inputs(hidden, weight)
+    return _LinearCrossEntropy.apply(hidden, weight, target.reshape(-1), vocab)
+
+
+def linear_distillation_loss(hidden, weight, top_values, top_indices, temperature=1.0, vocab=None):
+    """`distillation_loss` of the language-model head from its hidden rows, without the logits in memory; hidden and weight as for
+    `linear_cross_entropy`, top_values and top_indices [..., k]."""
+    hidden, weight = _head_inputs(hidden, weight)
+    k = top_indices.shape[-1]
+    return _LinearDistillation.apply(hidden, weight, top_values.detach().reshape(-1, k), top_indices.reshape(-1, k), temperature, vocab)
+
+
+def distillation_loss(logits, top_values, top_indices, temperature=1.0, vocab=None):
+    """Mean over rows of T^2 KL(q || softmax(logits / T)), q = softmax(top_values / T) over a teacher's top entries (torch.topk of its logits:
+    top_values [rows, k], top_indices [rows, k] int64; an index that names no class does not count, a row without entries is ignored).
+    logits [rows, cols] float32, float16 or bfloat16, columns from `vocab` on are padding.  No gradient goes to the teacher."""
+    return _Distillation.apply(logits, top_values.detach(), top_indices, temperature, vocab)
 
 
 class _LayerNormFunction(torch.autograd.Function):

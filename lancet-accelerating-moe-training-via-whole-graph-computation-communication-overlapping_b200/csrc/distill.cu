@@ -1,0 +1,277 @@
+// Distillation from a teacher's top logits on the student's (padded, 16-bit or float32) logits, forward and backward: the soft-target
+// counterpart of the cross entropy in xent.cu, on the same logits.  With q = softmax(v / T) over the teacher's k entries (v_i, idx_i) of a
+// row and z the student's logits,
+//     loss[r]   = T^2 sum_i q_i (log q_i - (z[r, idx_i] / T - lse[r])),      lse[r] = log sum_j exp(z[r, j] / T)
+//     dz[r, j]  = T (exp(z[r, j] / T - lse[r]) - sum_{i: idx_i = j} q_i) * g     (0 in rows without a teacher and in padded columns)
+// The teacher's tail is not modelled: its top entries are renormalised.  Both passes are bound by HBM: one read of the logits forward, one
+// read and one write backward; q is kept (k numbers per row), the logits' log-probabilities are not.
+#include "head_loss.cuh"
+
+#include <cfloat>
+
+namespace lancet {
+namespace head {
+
+__global__ void __launch_bounds__(kMeanThreads)
+mean_kernel(const float* __restrict__ loss_rows, const int32_t* __restrict__ live_rows, const int32_t* __restrict__ count, int rows,
+            float* __restrict__ mean, float* __restrict__ inv_live) {
+  chain_enter();
+  __shared__ double s_sum[kMeanThreads / 32];
+  __shared__ int s_live[kMeanThreads / 32];
+  double sum = 0.0;
+  int live = 0;
+  for (int r = threadIdx.x; r < rows; r += kMeanThreads) {
+    sum += (double)loss_rows[r];
+    if (live_rows) live += live_rows[r];
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    live += __shfl_xor_sync(0xffffffffu, live, d);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    s_sum[threadIdx.x >> 5] = sum;
+    s_live[threadIdx.x >> 5] = live;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double total = 0.0;
+    int n = 0;
+    for (int w = 0; w < kMeanThreads / 32; ++w) {
+      total += s_sum[w];
+      n += s_live[w];
+    }
+    if (count) n = *count;
+    n = n > 1 ? n : 1;
+    *mean = (float)(total / n);
+    *inv_live = 1.0f / (float)n;
+  }
+}
+
+int launch_mean(const float* loss_rows, const int32_t* live_rows, const int32_t* count, int rows, float* mean, float* inv_live, cudaStream_t st) {
+  launch_chained(mean_kernel, dim3(1), dim3(kMeanThreads), 0, st, loss_rows, live_rows, count, rows, mean, inv_live);
+  return launch_status("mean_kernel");
+}
+
+constexpr int kThreads = 256;
+
+template <typename T>
+struct alignas(16) Vec {
+  static constexpr int N = 16 / sizeof(T);
+  T v[N];
+};
+
+// Elements of a row before the first 16-byte boundary (the whole row where T's own alignment is all there is to have).
+template <typename T>
+__device__ __forceinline__ int row_head(const T* row, int n) {
+  const int head = (int)(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T));
+  return head < n ? head : n;
+}
+
+// Running maximum m (of the raw values, so that masks of the type's lowest value stay finite) and sum s of 2^((x - m) c).  m starts at
+// the lowest finite float: a value of -inf then adds 0, and a row of nothing but -inf ends with s = 0.
+__device__ __forceinline__ void add_one(float& m, float& s, float x, float c) {
+  if (x > m) {
+    s = s * ex2f((m - x) * c) + 1.0f;
+    m = x;
+  } else {
+    s += ex2f((x - m) * c);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void add_vec(float& m, float& s, const Vec<T>& a, float c) {
+  constexpr int N = Vec<T>::N;
+  float x[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) x[j] = Num<T>::to_f(a.v[j]);
+  float vm = x[0];
+#pragma unroll
+  for (int j = 1; j < N; ++j) vm = fmaxf(vm, x[j]);
+  if (vm > m) {
+    s *= ex2f((m - vm) * c);
+    m = vm;
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) s += ex2f((x[j] - m) * c);
+}
+__device__ __forceinline__ void merge(float& m, float& s, float m2, float s2, float c) {
+  const float mm = fmaxf(m, m2);
+  s = s * ex2f((m - mm) * c) + s2 * ex2f((m2 - mm) * c);
+  m = mm;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+distill_fwd_kernel(const T* __restrict__ x, long long ld, const void* __restrict__ values, int vdtype, const long long* __restrict__ indices,
+                   int k, float inv_t, int V, float* __restrict__ loss, float* __restrict__ lse, float* __restrict__ weights,
+                   int32_t* __restrict__ live_rows) {
+  chain_enter();
+  constexpr int N = Vec<T>::N;
+  __shared__ float s_q[kMaxTop];
+  __shared__ int s_idx[kMaxTop];
+  __shared__ float s_m[kThreads / 32], s_s[kThreads / 32];
+  __shared__ int s_live;
+  const long long r = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float c = inv_t * kLog2e;
+  if (warp == 0) {
+    const bool live = teacher_row(values, vdtype, indices, r, k, inv_t, V, s_q, s_idx);
+    if (lane == 0) s_live = live;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < k; i += kThreads) weights[r * k + i] = class_weight(s_q, s_idx, k, i);
+  if (!s_live) {
+    if (threadIdx.x == 0) {
+      loss[r] = 0.f;
+      lse[r] = 0.f;
+      live_rows[r] = 0;
+    }
+    return;
+  }
+  const T* row = x + r * ld;
+  float m = -FLT_MAX, s = 0.f;
+  const int head = row_head(row, V);
+  if ((int)threadIdx.x < head) add_one(m, s, Num<T>::to_f(row[threadIdx.x]), c);
+  const int nv = (V - head) / N;
+  const Vec<T>* rv = reinterpret_cast<const Vec<T>*>(row + head);
+  int i = threadIdx.x;
+  for (; i + 3 * kThreads < nv; i += 4 * kThreads) {   // four loads in flight
+    const Vec<T> a = rv[i], b = rv[i + kThreads], d = rv[i + 2 * kThreads], e = rv[i + 3 * kThreads];
+    add_vec(m, s, a, c);
+    add_vec(m, s, b, c);
+    add_vec(m, s, d, c);
+    add_vec(m, s, e, c);
+  }
+  for (; i < nv; i += kThreads) add_vec(m, s, rv[i], c);
+  for (int j = head + nv * N + threadIdx.x; j < V; j += kThreads) add_one(m, s, Num<T>::to_f(row[j]), c);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, d), s2 = __shfl_xor_sync(0xffffffffu, s, d);
+    merge(m, s, m2, s2, c);
+  }
+  if (lane == 0) {
+    s_m[warp] = m;
+    s_s[warp] = s;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    float M = s_m[0], S = s_s[0];
+    for (int w = 1; w < kThreads / 32; ++w) merge(M, S, s_m[w], s_s[w], c);
+    const float l = M * inv_t + logf(S);
+    float sum = 0.f;
+    for (int e = lane; e < k; e += 32)
+      if (s_q[e] != 0.f) sum += s_q[e] * (logf(s_q[e]) - (Num<T>::to_f(row[s_idx[e]]) * inv_t - l));
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) {
+      lse[r] = l;
+      loss[r] = sum / (inv_t * inv_t);
+      live_rows[r] = 1;
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+distill_bwd_kernel(const T* __restrict__ x, long long ld, const long long* __restrict__ indices, const float* __restrict__ weights,
+                   const int32_t* __restrict__ live_rows, int k, float inv_t, int V, int cols, const float* __restrict__ lse,
+                   const float* __restrict__ gout, const float* __restrict__ inv_live, float scale, T* __restrict__ dx, long long ldd) {
+  chain_enter();
+  constexpr int N = Vec<T>::N;
+  const long long r = blockIdx.x;
+  const T* row = x + r * ld;
+  T* drow = dx + r * ldd;
+  if (!live_rows[r]) {
+    for (int j = threadIdx.x; j < cols; j += kThreads) drow[j] = Num<T>::from_f(0.f);
+    return;
+  }
+  const float g = scale * (gout ? *gout : 1.f) * (inv_live ? *inv_live : 1.f) / inv_t;
+  const float c = inv_t * kLog2e, l = lse[r] / inv_t;   // differences of raw values, as in the forward pass
+  // vectors where both rows meet 16-byte boundaries at the same element
+  const bool same = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(drow)) & 15) == 0;
+  const int head = same ? row_head(row, V) : V;
+  const int nv = (V - head) / N;
+  const Vec<T>* rv = reinterpret_cast<const Vec<T>*>(row + head);
+  Vec<T>* dv = reinterpret_cast<Vec<T>*>(drow + head);
+  auto grad = [&](float v) { return Num<T>::from_f(ex2f((v - l) * c) * g); };
+  auto grad_vec = [&](const Vec<T>& a) {
+    Vec<T> o;
+#pragma unroll
+    for (int j = 0; j < N; ++j) o.v[j] = grad(Num<T>::to_f(a.v[j]));
+    return o;
+  };
+  for (int j = threadIdx.x; j < head; j += kThreads) drow[j] = grad(Num<T>::to_f(row[j]));
+  int i = threadIdx.x;
+  for (; i + 3 * kThreads < nv; i += 4 * kThreads) {
+    const Vec<T> a0 = rv[i], a1 = rv[i + kThreads], a2 = rv[i + 2 * kThreads], a3 = rv[i + 3 * kThreads];
+    dv[i] = grad_vec(a0);
+    dv[i + kThreads] = grad_vec(a1);
+    dv[i + 2 * kThreads] = grad_vec(a2);
+    dv[i + 3 * kThreads] = grad_vec(a3);
+  }
+  for (; i < nv; i += kThreads) dv[i] = grad_vec(rv[i]);
+  for (int j = head + nv * N + threadIdx.x; j < cols; j += kThreads) drow[j] = j < V ? grad(Num<T>::to_f(row[j])) : Num<T>::from_f(0.f);
+  __syncthreads();
+  // the teacher's classes: difference in float32, rounded once (entries of one class write the same value)
+  for (int e = threadIdx.x; e < k; e += kThreads) {
+    const long long at = indices[r * k + e];
+    if (at >= 0 && at < V) drow[at] = Num<T>::from_f((ex2f((Num<T>::to_f(row[at]) - l) * c) - weights[r * k + e]) * g);
+  }
+}
+
+template <typename T>
+static int fwd_t(const void* x, long long ld, const void* values, int vdtype, const long long* indices, int k, float inv_t, int rows, int vocab,
+                 float* loss, float* lse, float* weights, int32_t* live_rows, cudaStream_t st) {
+  launch_chained(distill_fwd_kernel<T>, dim3(rows), dim3(kThreads), 0, st, static_cast<const T*>(x), ld, values, vdtype, indices, k, inv_t,
+                 vocab, loss, lse, weights, live_rows);
+  return launch_status("distill_fwd_kernel");
+}
+
+template <typename T>
+static int bwd_t(const void* x, long long ld, const long long* indices, const float* weights, const int32_t* live_rows, int k, float inv_t,
+                 int rows, int vocab, int cols, const float* lse, const float* gout, const float* inv_live, float scale, void* dx,
+                 long long ldd, cudaStream_t st) {
+  launch_chained(distill_bwd_kernel<T>, dim3(rows), dim3(kThreads), 0, st, static_cast<const T*>(x), ld, indices, weights, live_rows, k,
+                 inv_t, vocab, cols, lse, gout, inv_live, scale, static_cast<T*>(dx), ldd);
+  return launch_status("distill_bwd_kernel");
+}
+
+}  // namespace head
+}  // namespace lancet
+
+extern "C" {
+using namespace lancet;
+
+int lancet_distill_fwd(const void* logits, long long ld, const void* top_values, int values_dtype, const long long* top_indices, int k,
+                       float temperature, int rows, int vocab, int dtype, float* loss_rows, float* lse_rows, float* class_weights,
+                       int32_t* live_rows, float* mean, float* inv_live, lancet_stream_t stream) {
+  LANCET_REQUIRE(rows >= 0 && vocab >= 1 && ld >= vocab && valid_dtype(dtype) && valid_dtype(values_dtype), LANCET_ERR_INVALID,
+                 "lancet_distill_fwd: bad rows=%d, vocab=%d, row stride %lld or dtype", rows, vocab, ld);
+  LANCET_REQUIRE(k >= 1 && k <= head::kMaxTop, LANCET_ERR_INVALID, "lancet_distill_fwd: k=%d top entries (1 to %d)", k, head::kMaxTop);
+  LANCET_REQUIRE(temperature >= 1e-3f && temperature <= 1e3f, LANCET_ERR_INVALID, "lancet_distill_fwd: temperature %g outside [0.001, 1000]",
+                 (double)temperature);
+  LANCET_REQUIRE(mean && inv_live && (rows == 0 || (logits && top_values && top_indices && loss_rows && lse_rows && class_weights && live_rows)),
+                 LANCET_ERR_NULL, "lancet_distill_fwd: null pointer argument");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rows > 0)
+    if (int rc = LANCET_DISPATCH_DTYPE(dtype, head::fwd_t, logits, ld, top_values, values_dtype, top_indices, k, 1.0f / temperature, rows,
+                                       vocab, loss_rows, lse_rows, class_weights, live_rows, st))
+      return rc;
+  return head::launch_mean(loss_rows, live_rows, nullptr, rows, mean, inv_live, st);
+}
+
+int lancet_distill_bwd(const void* logits, long long ld, const long long* top_indices, const float* class_weights, const int32_t* live_rows,
+                       int k, float temperature, int rows, int vocab, int cols, int dtype, const float* lse_rows, const float* grad_out,
+                       const float* inv_live, float scale, void* dlogits, long long ldd, lancet_stream_t stream) {
+  LANCET_REQUIRE(rows >= 0 && vocab >= 1 && cols >= vocab && ld >= vocab && ldd >= cols && valid_dtype(dtype), LANCET_ERR_INVALID,
+                 "lancet_distill_bwd: bad rows=%d, vocab=%d, cols=%d, row strides %lld / %lld or dtype", rows, vocab, cols, ld, ldd);
+  LANCET_REQUIRE(k >= 1 && k <= head::kMaxTop, LANCET_ERR_INVALID, "lancet_distill_bwd: k=%d top entries (1 to %d)", k, head::kMaxTop);
+  LANCET_REQUIRE(temperature >= 1e-3f && temperature <= 1e3f, LANCET_ERR_INVALID, "lancet_distill_bwd: temperature %g outside [0.001, 1000]",
+                 (double)temperature);
+  if (rows == 0) return LANCET_OK;
+  LANCET_REQUIRE(logits && top_indices && class_weights && live_rows && lse_rows && dlogits, LANCET_ERR_NULL,
+                 "lancet_distill_bwd: null pointer argument");
+  return LANCET_DISPATCH_DTYPE(dtype, head::bwd_t, logits, ld, top_indices, class_weights, live_rows, k, 1.0f / temperature, rows, vocab, cols,
+                               lse_rows, grad_out, inv_live, scale, dlogits, ldd, static_cast<cudaStream_t>(stream));
+}
+}

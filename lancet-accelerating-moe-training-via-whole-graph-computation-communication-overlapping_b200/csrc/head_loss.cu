@@ -1,0 +1,1008 @@
+// Losses of the language-model head from its hidden rows, without keeping the logits: cross entropy against target tokens and distillation
+// from a teacher's top logits, forward and backward.  With h [rows][width], W [classes][width] and z = h W^T (never in memory as a whole),
+//     lse[r]  = log sum_j exp(z[r, j] / T)                         (T = 1 for the cross entropy)
+//     loss[r] = lse[r] - z[r, t_r]          or   T^2 sum_i q_i (log q_i - (z[r, idx_i] / T - lse[r])),   q = softmax(v / T)
+//     dz[r, j] = T (exp(z[r, j] / T - lse[r]) - sum_{i: idx_i = j} q_i) g,     dh = dz W,     dW = dz^T h      (one entry with q = 1 for a target)
+// The forward pass is one product whose epilogue reduces each tile's columns to a running maximum and sum per row.  The backward pass walks
+// the vocabulary in pieces: the same product again with an epilogue that writes exp(z / T - lse) of the piece in 16 bits, a small kernel
+// that puts the differences at the targets in place, and two products from that piece.  2 + 2 + 4 flops per row, class and width element.
+//
+// Rows without a target (or teacher) take no part: a first kernel packs the live rows together (dense rows, zeros up to the next tile
+// boundary), every product works on their number, which stays on the device, and the gradient rows go back through the row list.  So an
+// ignored row may hold anything, NaN included, and costs a copy's time only.
+//
+// All products run on one kernel: tcgen05.mma from 128-byte-swizzled tiles staged by TMA, float32 accumulators in TMEM, two of them so that
+// the epilogue of one tile runs under the next tile's products.
+#include "head_loss.cuh"
+#include "tcgen05.cuh"
+
+namespace lancet {
+namespace head {
+
+using namespace lancet::gemm;
+
+constexpr int BM = 128, BN = 256, BK = 64, UMMA_K = 16;
+constexpr int A_STAGE_BYTES = BM * BK * 2;
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int TMEM_COLS = 512;
+constexpr int ROW_PAD = 256;                    // packed rows are padded with zeros to a multiple of this
+constexpr long long BAND_BYTES = 20ll << 20;    // rows of A swept against all columns before the next band: they stay in L2
+
+// Products (A's and B's rows are M and N):
+//   FORM_Z   z tile  = h W^T       M = live rows, N = classes, reduction over the width;    both operands K-major
+//   FORM_DH  dh tile = dz W        M = live rows, N = width, reduction over the classes;    W is MN-major
+//   FORM_DW  dW tile = dz^T h      M = classes, N = width, reduction over the live rows;    both MN-major
+constexpr int FORM_Z = 0, FORM_DH = 1, FORM_DW = 2;
+constexpr int EPI_LSE = 0, EPI_PROB = 1, EPI_OUT = 2;
+
+template <bool CTA2>
+struct Cfg {
+  static constexpr int STAGES = CTA2 ? 6 : 4;
+  static constexpr int B_COLS = CTA2 ? BN / 2 : BN;
+  static constexpr int B_STAGE_BYTES = B_COLS * BK * 2;
+  static constexpr int STAGE_BYTES = A_STAGE_BYTES + B_STAGE_BYTES;
+  static constexpr int SMEM_DATA = STAGES * STAGE_BYTES;
+  static constexpr int SMEM_BYTES = SMEM_DATA + 1024 + 256;
+};
+
+struct Params {
+  const int32_t* count;   // live rows
+  int classes;            // of this piece
+  int class0;             // first class of the piece
+  int width;
+  int* status;
+  float c;                // log2(e) / T
+  // EPI_LSE: per (column half tile, row) maximum and sum in the base-2 domain
+  float2* part;
+  long long part_ld;
+  // EPI_PROB: 2^(z c - lse2[row] + shift) of the piece
+  const float* lse2;
+  float shift;
+  void* dz;
+  long long dz_ld;
+  // EPI_OUT
+  void* out;
+  const int32_t* row_map;   // output row of packed row i, or null
+  const float* grad_out;
+  const float* inv_live;
+  float scale;
+  float* acc;               // float32 sums over the pieces, or null
+  int acc_in, acc_out;      // add the sums so far / store sums instead of the output
+};
+
+struct Dims {
+  int m, n, k;      // k: length of the reduction
+  int mu, nt, kb;   // units of rows (a tile, or a pair's two), column tiles, blocks of the reduction
+};
+template <int FORM, bool CTA2>
+__device__ __forceinline__ Dims dims_of(const Params& p) {
+  Dims d;
+  const int rows = *p.count;
+  d.m = FORM == FORM_DW ? p.classes : rows;
+  d.n = FORM == FORM_Z ? p.classes : p.width;
+  d.k = FORM == FORM_Z ? p.width : (FORM == FORM_DH ? p.classes : rows);
+  const int unit = CTA2 ? 2 * BM : BM;
+  d.mu = (d.m + unit - 1) / unit;
+  d.nt = (d.n + BN - 1) / BN;
+  d.kb = (d.k + BK - 1) / BK;
+  return d;
+}
+
+struct Tile {
+  int mt, nt;   // this CTA's 128-row tile, column tile
+};
+// FORM_Z: bands of row units that stay in L2, swept against the column tiles.  Otherwise the index with fewer tiles runs fastest: the tiles
+// in flight form a block as square as possible and share the most operand slabs.
+template <int FORM, bool CTA2>
+__device__ __forceinline__ Tile decode(const Params& p, const Dims& d, int t, int rank) {
+  int mu, nt;
+  if (FORM == FORM_Z) {
+    const long long unit_bytes = (long long)(CTA2 ? 2 * BM : BM) * p.width * 2;
+    int band = (int)(BAND_BYTES / unit_bytes);
+    band = band < 2 ? 2 : band;
+    const int b = t / (band * d.nt);
+    const int in_band = min(band, d.mu - b * band);
+    const int r = t - b * band * d.nt;
+    nt = r / in_band;
+    mu = b * band + (r - nt * in_band);
+  } else if (d.nt < d.mu) {
+    mu = t / d.nt;
+    nt = t - mu * d.nt;
+  } else {
+    nt = t / d.mu;
+    mu = t - nt * d.mu;
+  }
+  Tile tl;
+  tl.mt = CTA2 ? 2 * mu + rank : mu;
+  tl.nt = nt;
+  return tl;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <typename T, int FORM, int EPI, bool CTA2>
+__global__ void __launch_bounds__(THREADS, 1)
+head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, Params p) {
+  using C = Cfg<CTA2>;
+  constexpr int STAGES = C::STAGES;
+  constexpr bool A_MN = FORM == FORM_DW, B_MN = FORM != FORM_Z;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char* sA = smem;
+  unsigned char* sB = smem + STAGES * A_STAGE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::SMEM_DATA);
+  const uint32_t bar_full = smem_u32(bars), bar_empty = smem_u32(bars + STAGES);
+  const uint32_t bar_tfull = smem_u32(bars + 2 * STAGES), bar_tempty = smem_u32(bars + 2 * STAGES + 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = CTA2 ? (int)cluster_ctarank() : 0;
+  const int worker = CTA2 ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
+  const int n_workers = CTA2 ? (int)(gridDim.x >> 1) : (int)gridDim.x;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar_tfull + 8 * b, 1);
+      mbar_init(bar_tempty + 8 * b, CTA2 ? 2 * EPI_WARPS : EPI_WARPS);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    if (CTA2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (CTA2) cluster_sync_all();   // the peer's barriers exist before anything signals them
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  chain_enter();                  // the set-up above overlaps the previous kernel's end; its results are read from here on
+  const Dims d = dims_of<FORM, CTA2>(p);
+  const int n_tiles = d.mu * d.nt;
+
+  if (warp == 0) {
+    // ---------------- TMA producer (one per CTA; in the paired form each CTA loads its own halves) ----------------
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const int b_off = CTA2 ? rank * (BN / 2) : 0;   // this CTA's share of the tile's columns
+      for (int t = worker; t < n_tiles && ok; t += n_workers) {
+        const Tile tl = decode<FORM, CTA2>(p, d, t, rank);
+        const int m0 = tl.mt * BM, n0 = tl.nt * BN + b_off;
+        for (int kb = 0; kb < d.kb; ++kb) {
+          if (!(ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.status, 11))) break;
+          const uint32_t a_dst = smem_u32(sA + stage * A_STAGE_BYTES), b_dst = smem_u32(sB + stage * C::B_STAGE_BYTES);
+          uint32_t full = bar_full + 8 * stage;
+          if (rank == 0) mbar_expect_tx(full, (CTA2 ? 2 : 1) * C::STAGE_BYTES);   // of a pair: both CTAs' bytes
+          if (CTA2) full = cluster_addr(full, 0);
+          auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
+            if (CTA2) tma_load_2d_pair(dst, map, full, x, y); else tma_load_2d(dst, map, full, x, y);
+          };
+          if (!A_MN) {
+            load(a_dst, &tmA, kb * BK, m0);
+          } else {
+#pragma unroll
+            for (int j = 0; j < BM / 64; ++j) load(a_dst + j * BOX_BYTES, &tmA, m0 + j * 64, kb * BK);
+          }
+          if (!B_MN) {
+            load(b_dst, &tmB, kb * BK, p.class0 + n0);
+          } else {
+            const int y = (FORM == FORM_DH ? p.class0 : 0) + kb * BK;
+#pragma unroll
+            for (int j = 0; j < C::B_COLS / 64; ++j) load(b_dst + j * BOX_BYTES, &tmB, n0 + j * 64, y);
+          }
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (paired form: the even CTA only) ----------------
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = instr_desc<T>(A_MN, B_MN, CTA2 ? 2 * BM : BM, BN);
+      int stage = 0;
+      uint32_t phase = 0;
+      int buf = 0;
+      uint32_t tphase[2] = {0, 0};
+      bool ok = true;
+      for (int t = worker; t < n_tiles && ok; t += n_workers) {
+        if (!(ok = mbar_wait(bar_tempty + 8 * buf, tphase[buf] ^ 1, abort_flag, p.status, 12))) break;
+        tc_fence_after();
+        const uint32_t tmem_d = tmem_base + (uint32_t)(buf * BN);
+        for (int kb = 0; kb < d.kb; ++kb) {
+          if (!(ok = mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, 13))) break;
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(sA + stage * A_STAGE_BYTES);
+          const uint32_t b_addr = smem_u32(sB + stage * C::B_STAGE_BYTES);
+#pragma unroll
+          for (int k = 0; k < BK / UMMA_K; ++k) {
+            const uint64_t adesc = A_MN ? smem_desc_mn_sw128(a_addr + k * 2048) : smem_desc_k_sw128(a_addr + k * UMMA_K * 2);
+            const uint64_t bdesc = B_MN ? smem_desc_mn_sw128(b_addr + k * 2048) : smem_desc_k_sw128(b_addr + k * UMMA_K * 2);
+            if (CTA2)
+              umma_f16_pair(tmem_d, adesc, bdesc, idesc, (kb | k) ? 1u : 0u);
+            else
+              umma_f16(tmem_d, adesc, bdesc, idesc, (kb | k) ? 1u : 0u);
+          }
+          if (CTA2) umma_commit_pair(bar_empty + 8 * stage); else umma_commit(bar_empty + 8 * stage);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        if (CTA2) umma_commit_pair(bar_tfull + 8 * buf); else umma_commit(bar_tfull + 8 * buf);
+        tphase[buf] ^= 1;
+        buf ^= 1;
+      }
+    }
+  } else {
+    // ---------------- epilogue: TMEM lane quadrant = warp % 4, column half = (warp - 2) / 4; a thread owns one row ----------------
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    constexpr int CHUNKS = BN / 64;   // 32-column chunks of a half tile
+    int buf = 0;
+    uint32_t tphase[2] = {0, 0};
+    bool ok = true;
+    float g = 1.f;
+    if (EPI == EPI_OUT) g = p.scale * (p.grad_out ? *p.grad_out : 1.f) * (p.inv_live ? *p.inv_live : 1.f);
+    const uint32_t acc_mask = d.kb > 0 ? 0xffffffffu : 0u;   // no live rows: the accumulator holds stale values
+    for (int t = worker; t < n_tiles && ok; t += n_workers) {
+      const Tile tl = decode<FORM, CTA2>(p, d, t, rank);
+      const int row = tl.mt * BM + quad * 32 + lane;
+      const bool row_live = row < d.m;
+      const int col_first = tl.nt * BN + half * (BN / 2);
+      float off = 0.f;
+      long long out_row = row;
+      if (EPI == EPI_PROB && row_live) off = p.shift - p.lse2[row];
+      if (EPI == EPI_OUT && row_live) out_row = p.row_map ? (p.acc_out ? row : p.row_map[row]) : (long long)p.class0 + row;
+      ok = mbar_wait(bar_tfull + 8 * buf, tphase[buf], abort_flag, p.status, 14);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN + half * (BN / 2));
+      float m = -1e30f, s = 0.f;   // EPI_LSE: maximum of z and sum of 2^((z - m) c)
+#pragma unroll 1
+      for (int ch = 0; ch < CHUNKS; ++ch) {
+        uint32_t r[32];
+        tmem_ld32(taddr + ch * 32, r);
+        const int left = d.n - (col_first + ch * 32);   // columns of the chunk that exist
+        if (EPI == EPI_LSE) {
+          if (left < 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = i < left ? r[i] : 0xff800000u;
+          }
+          float mx = __uint_as_float(r[0]);
+#pragma unroll
+          for (int i = 1; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
+          mx = fmaxf(mx, m);
+          s *= ex2f((m - mx) * p.c);
+          m = mx;
+          const float mc = -m * p.c;
+          float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s4[i & 3] += ex2f(fmaf(__uint_as_float(r[i]), p.c, mc));
+          s += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+        } else if (EPI == EPI_PROB) {
+          uint32_t o[16];
+          const uint32_t keep = row_live ? 0xffffffffu : 0u;
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float a = ex2f(fmaf(__uint_as_float(r[i]), p.c, off)), b = ex2f(fmaf(__uint_as_float(r[i + 1]), p.c, off));
+            if (left < 32) {
+              a = i < left ? a : 0.f;
+              b = i + 1 < left ? b : 0.f;
+            }
+            o[i >> 1] = pack_pair<T>(a, b) & keep;
+          }
+          // the piece's buffer has whole tiles: every row and column of this one is written, zeros behind the last live ones
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.dz) + row * p.dz_ld + col_first + ch * 32);
+#pragma unroll
+          for (int q = 0; q < 4; q += 2)
+            st_global_32B(dst + q, make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]),
+                          make_uint4(o[4 * q + 4], o[4 * q + 5], o[4 * q + 6], o[4 * q + 7]));
+        } else if (row_live && left > 0) {
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i] & acc_mask);
+          if (p.acc && p.acc_in) {
+            const float* a = p.acc + (long long)row * p.width + col_first + ch * 32;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] += i < left ? a[i] : 0.f;
+          }
+          if (p.acc && p.acc_out) {
+            float* a = p.acc + (long long)row * p.width + col_first + ch * 32;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i < left) a[i] = v[i];
+          } else {
+            T* dst = static_cast<T*>(p.out) + out_row * p.width + col_first + ch * 32;
+            if (left >= 32 && (reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
+              uint32_t o[16];
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) o[i >> 1] = pack_pair<T>(v[i] * g, v[i + 1] * g);
+#pragma unroll
+              for (int q = 0; q < 4; q += 2)
+                st_global_32B(dst + 8 * q, make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]),
+                              make_uint4(o[4 * q + 4], o[4 * q + 5], o[4 * q + 6], o[4 * q + 7]));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (i < left) dst[i] = Num<T>::from_f(v[i] * g);
+            }
+          }
+        }
+      }
+      if (EPI == EPI_LSE && row_live) p.part[(long long)(2 * tl.nt + half) * p.part_ld + row] = make_float2(m * p.c, s);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (CTA2) mbar_arrive_cluster(cluster_addr(bar_tempty + 8 * buf, 0)); else mbar_arrive(bar_tempty + 8 * buf);
+      }
+      tphase[buf] ^= 1;
+      buf ^= 1;
+    }
+  }
+  // ---------------- teardown ----------------
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    // a wait gave up: let TMA copies that may still be in flight land before the CTA goes away
+    const unsigned long long t0 = now_ns();
+    while (now_ns() - t0 < 200000ull) {
+    }
+    __syncthreads();
+  }
+  if (CTA2) cluster_sync_all();   // the peer no longer signals this CTA's barriers or reads its shared memory
+  if (warp == 1) {
+    tc_fence_after();
+    if (CTA2)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+  }
+}
+
+// ---- live rows ------------------------------------------------------------------------------------------------------------
+constexpr int kRowThreads = 256;
+
+// One row of 16-bit elements by one warp, 16 bytes a lane where both ends allow it.  src null: zeros.
+__device__ __forceinline__ void copy_row(uint16_t* dst, const uint16_t* src, int width) {
+  const int lane = threadIdx.x & 31;
+  const bool vec = ((reinterpret_cast<uintptr_t>(dst) | reinterpret_cast<uintptr_t>(src)) & 15) == 0;
+  const int nv = vec ? width / 8 : 0;
+  for (int i = lane; i < nv; i += 32)
+    reinterpret_cast<uint4*>(dst)[i] = src ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0);
+  for (int i = nv * 8 + lane; i < width; i += 32) dst[i] = src ? src[i] : (uint16_t)0;
+}
+
+__device__ __forceinline__ bool row_is_live(const long long* target, const int32_t* flags, int r, int vocab) {
+  if (flags) return flags[r] != 0;
+  const long long t = target[r];
+  return t >= 0 && t < vocab;
+}
+
+// Packs the live rows: pos[r] = packed index of row r or -1, pos[rows] = their number, packed rows, zero rows up to the next multiple of
+// ROW_PAD.  Each block owns a range of rows and first counts the live rows before it.
+__global__ void __launch_bounds__(kRowThreads)
+pack_rows_kernel(const uint16_t* __restrict__ hidden, long long ld, const long long* __restrict__ target, const int32_t* __restrict__ flags,
+                 int rows, int vocab, int width, uint16_t* __restrict__ packed, int packed_ld, int32_t* __restrict__ origin,
+                 int32_t* __restrict__ pos, float* __restrict__ loss_rows, float* __restrict__ lse_rows) {
+  chain_enter();
+  __shared__ int s_warp[kRowThreads / 32];
+  __shared__ int s_at[kRowThreads];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per = (rows + gridDim.x - 1) / gridDim.x;
+  const int r0 = min(rows, (int)blockIdx.x * per), r1 = min(rows, r0 + per);
+  int before = 0;
+  for (int r = threadIdx.x; r < r0; r += kRowThreads) before += row_is_live(target, flags, r, vocab);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
+  if (lane == 0) s_warp[warp] = before;
+  __syncthreads();
+  before = 0;
+  for (int w = 0; w < kRowThreads / 32; ++w) before += s_warp[w];
+  for (int base = r0; base < r1; base += kRowThreads) {
+    __syncthreads();
+    const int r = base + threadIdx.x;
+    const bool live = r < r1 && row_is_live(target, flags, r, vocab);
+    const unsigned ballot = __ballot_sync(0xffffffffu, live);
+    if (lane == 0) s_warp[warp] = __popc(ballot);
+    __syncthreads();
+    int at = before;
+    for (int w = 0; w < warp; ++w) at += s_warp[w];
+    at += __popc(ballot & ((1u << lane) - 1));
+    if (r < r1) {
+      pos[r] = live ? at : -1;
+      if (live) {
+        origin[at] = r;
+      } else {
+        loss_rows[r] = 0.f;
+        lse_rows[r] = 0.f;
+      }
+    }
+    s_at[threadIdx.x] = live ? at : -1;
+    __syncthreads();
+    for (int i = warp; i < min(kRowThreads, r1 - base); i += kRowThreads / 32)
+      if (s_at[i] >= 0) copy_row(packed + (long long)s_at[i] * packed_ld, hidden + (long long)(base + i) * ld, width);
+    for (int w = 0; w < kRowThreads / 32; ++w) before += s_warp[w];
+  }
+  if (blockIdx.x == gridDim.x - 1) {
+    if (threadIdx.x == 0) pos[rows] = before;
+    const int end = (before + ROW_PAD - 1) / ROW_PAD * ROW_PAD;
+    for (int i = before + warp; i < end; i += kRowThreads / 32) copy_row(packed + (long long)i * packed_ld, nullptr, width);
+  }
+}
+
+// The same packing in the backward pass, from pos; gradient rows of ignored rows are zeroed, lse goes to packed order and base 2.
+__global__ void __launch_bounds__(kRowThreads)
+repack_rows_kernel(const uint16_t* __restrict__ hidden, long long ld, const int32_t* __restrict__ pos, const float* __restrict__ lse_rows,
+                   int rows, int width, uint16_t* __restrict__ packed, int packed_ld, int32_t* __restrict__ origin, float* __restrict__ lse2,
+                   uint16_t* __restrict__ dhidden) {
+  chain_enter();
+  const int lane = threadIdx.x & 31;
+  const int warps = gridDim.x * (kRowThreads / 32);
+  const int first = blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
+  for (int r = first; r < rows; r += warps) {
+    const int at = pos[r];
+    if (at >= 0) {
+      copy_row(packed + (long long)at * packed_ld, hidden + (long long)r * ld, width);
+      if (lane == 0) {
+        origin[at] = r;
+        lse2[at] = lse_rows[r] * kLog2e;
+      }
+    } else if (dhidden) {
+      copy_row(dhidden + (long long)r * width, nullptr, width);
+    }
+  }
+  const int count = pos[rows], end = (count + ROW_PAD - 1) / ROW_PAD * ROW_PAD;
+  for (int i = count + first; i < end; i += warps) copy_row(packed + (long long)i * packed_ld, nullptr, width);
+}
+
+// ---- row results ----------------------------------------------------------------------------------------------------------
+constexpr int kFinishThreads = 256;
+
+template <typename T>
+__device__ __forceinline__ float warp_dot(const T* a, const T* b, int width) {
+  const int lane = threadIdx.x & 31;
+  float s = 0.f;
+  // both rows start on 16-byte boundaries (packed rows; the weight's rows as the tensor map wants them)
+  const int nv = width / 8;
+  for (int i = lane; i < nv; i += 32) {
+    const uint4 x = reinterpret_cast<const uint4*>(a)[i], y = reinterpret_cast<const uint4*>(b)[i];
+    const T* xs = reinterpret_cast<const T*>(&x);
+    const T* ys = reinterpret_cast<const T*>(&y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fmaf(Num<T>::to_f(xs[j]), Num<T>::to_f(ys[j]), s);
+  }
+  for (int i = nv * 8 + lane; i < width; i += 32) s = fmaf(Num<T>::to_f(a[i]), Num<T>::to_f(b[i]), s);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  return s;
+}
+
+// A block finishes kRows packed rows: joins the partial maxima and sums of its rows' column half tiles (in tile order), then each warp
+// takes rows and computes the logits at their targets as dot products.  k entries per row: idx [rows][k] (-1: none), q and class weights
+// [rows][k]; or a target per row.
+template <typename T, int kRows>
+__global__ void __launch_bounds__(kFinishThreads)
+finish_rows_kernel(const float2* __restrict__ part, long long part_ld, int n_part, const int32_t* __restrict__ count,
+                   const int32_t* __restrict__ origin, const T* __restrict__ packed, int packed_ld, const T* __restrict__ weight,
+                   long long weight_ld, int width, const long long* __restrict__ target, const int32_t* __restrict__ idx,
+                   const float* __restrict__ q, const float* __restrict__ cw, int k, float inv_t, float* __restrict__ loss_rows,
+                   float* __restrict__ lse_rows, float* __restrict__ diff) {
+  chain_enter();
+  constexpr int G = kFinishThreads / kRows;
+  __shared__ float s_m[G][kRows], s_s[G][kRows];
+  __shared__ float s_lse[kRows];
+  const int n = *count;
+  const int base = blockIdx.x * kRows;
+  if (base >= n) return;
+  const int rr = threadIdx.x % kRows, grp = threadIdx.x / kRows;
+  float m = -INFINITY, s = 0.f;
+  if (base + rr < n) {
+    m = -1e38f;
+    for (int t = grp; t < n_part; t += G) {
+      const float2 v = part[(long long)t * part_ld + base + rr];
+      const float mm = fmaxf(m, v.x);
+      s = s * ex2f(m - mm) + v.y * ex2f(v.x - mm);
+      m = mm;
+    }
+  }
+  s_m[grp][rr] = m;
+  s_s[grp][rr] = s;
+  __syncthreads();
+  if (grp == 0 && base + rr < n) {
+    for (int j = 1; j < G; ++j) {
+      const float m2 = s_m[j][rr], mm = fmaxf(m, m2);
+      s = s * ex2f(m - mm) + s_s[j][rr] * ex2f(m2 - mm);
+      m = mm;
+    }
+    s_lse[rr] = m * kLn2 + logf(s);
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int i = warp; i < kRows && base + i < n; i += kFinishThreads / 32) {
+    const int c = base + i;
+    const long long r = origin[c];
+    const float lse = s_lse[i];
+    const T* h = packed + (long long)c * packed_ld;
+    if (target) {
+      const float z = warp_dot(h, weight + target[r] * weight_ld, width);
+      if (lane == 0) {
+        loss_rows[r] = lse - z;
+        lse_rows[r] = lse;
+      }
+    } else {
+      float sum = 0.f;
+      for (int e = 0; e < k; ++e) {
+        const long long at = r * k + e;
+        const int cls = idx[at];
+        if (cls < 0) continue;
+        const float lp = warp_dot(h, weight + (long long)cls * weight_ld, width) * inv_t - lse;
+        const float qe = q[at];
+        if (qe != 0.f) sum += qe * (logf(qe) - lp);
+        if (lane == 0) diff[at] = expf(lp) - cw[at];
+      }
+      if (lane == 0) {
+        loss_rows[r] = sum / (inv_t * inv_t);
+        lse_rows[r] = lse;
+      }
+    }
+  }
+}
+
+// Teacher distributions of all rows, a warp each: q, class weights, indices as int32 (-1: does not count), live flags.
+constexpr int kTeacherWarps = 4;
+__global__ void __launch_bounds__(32 * kTeacherWarps)
+teacher_kernel(const void* __restrict__ values, int vdtype, const long long* __restrict__ indices, int rows, int k, float inv_t, int vocab,
+               float* __restrict__ q, float* __restrict__ cw, int32_t* __restrict__ idx, int32_t* __restrict__ live) {
+  chain_enter();
+  __shared__ float s_q[kTeacherWarps][kMaxTop];
+  __shared__ int s_idx[kTeacherWarps][kMaxTop];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long r = (long long)blockIdx.x * kTeacherWarps + warp;
+  if (r >= rows) return;
+  const bool alive = teacher_row(values, vdtype, indices, r, k, inv_t, vocab, s_q[warp], s_idx[warp]);
+  if (lane == 0) live[r] = alive;
+  for (int i = lane; i < k; i += 32) {
+    q[r * k + i] = s_q[warp][i];
+    cw[r * k + i] = class_weight(s_q[warp], s_idx[warp], k, i);
+    idx[r * k + i] = s_idx[warp][i];
+  }
+}
+
+// dz at the targets of the piece: the difference in float32, rounded once.  Entries of one row that name the same class write the same value.
+template <typename T>
+__global__ void __launch_bounds__(256)
+place_targets_kernel(const int32_t* __restrict__ count, const int32_t* __restrict__ origin, const long long* __restrict__ target,
+                     const float* __restrict__ loss_rows, const long long* __restrict__ top_indices, const float* __restrict__ diff, int k,
+                     int class0, int classes, float unit, T* __restrict__ dz, long long dz_ld) {
+  chain_enter();
+  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  const long long c = i / k;
+  if (c >= *count) return;
+  const long long r = origin[c];
+  const long long e = r * k + (i - c * k);
+  const long long at = (target ? target[r] : top_indices[e]) - class0;
+  if (at < 0 || at >= classes) return;
+  const float v = target ? expm1f(-loss_rows[r]) : diff[e];
+  dz[c * dz_ld + at] = Num<T>::from_f(v * unit);
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------------
+static int make_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, int dtype) {
+  EncodeTiledFn fn = encode_fn();
+  LANCET_REQUIRE(fn, LANCET_ERR_CUDA, "head product: the driver does not provide cuTensorMapEncodeTiled");
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {ld * 2};
+  cuuint32_t box[2] = {(cuuint32_t)BK, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, dtype == LANCET_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                  const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  LANCET_REQUIRE(r == CUDA_SUCCESS, LANCET_ERR_CUDA, "head product: cuTensorMapEncodeTiled failed with code %d", (int)r);
+  return LANCET_OK;
+}
+
+// The paired form halves the bytes of B through shared memory per product; up to 128 rows its second tile would be empty.
+static bool paired_for(int m) { return m > BM; }
+
+template <typename T, int FORM, int EPI, bool CTA2>
+static int launch_form(const CUtensorMap& tmA, const CUtensorMap& tmB, const Params& p, long long units, cudaStream_t st) {
+  auto kernel = head_product_kernel<T, FORM, EPI, CTA2>;
+  constexpr int SMEM = Cfg<CTA2>::SMEM_BYTES;
+  static int set_for[64] = {0};   // per device
+  int dev = 0;
+  LANCET_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !__atomic_load_n(&set_for[dev], __ATOMIC_ACQUIRE)) {
+    LANCET_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    if (dev >= 0 && dev < 64) __atomic_store_n(&set_for[dev], 1, __ATOMIC_RELEASE);
+  }
+  long long grid = sm_count();
+  if (gemm_cta_limit() > 0 && gemm_cta_limit() < grid) grid = gemm_cta_limit();
+  if (grid > units * (CTA2 ? 2 : 1)) grid = units * (CTA2 ? 2 : 1);
+  if (CTA2) grid &= ~1ll;
+  if (grid < (CTA2 ? 2 : 1)) grid = CTA2 ? 2 : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = chained_launch_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CTA2 ? 2 : 1;
+  {
+    ProfScope prof("head_product_kernel", st);
+    cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, p);
+  }
+  return launch_status("head_product_kernel");
+}
+
+template <typename T, int FORM, int EPI>
+static int launch_product(const CUtensorMap& tmA, const CUtensorMap& tmB, const Params& p, int m, int n, bool paired, cudaStream_t st) {
+  const long long unit = paired ? 2 * BM : BM;
+  const long long units = ((m + unit - 1) / unit) * ((n + BN - 1) / BN);
+  LANCET_REQUIRE(units < (1ll << 30), LANCET_ERR_INVALID, "head product: %lld tiles", units);
+  return paired ? launch_form<T, FORM, EPI, true>(tmA, tmB, p, units, st) : launch_form<T, FORM, EPI, false>(tmA, tmB, p, units, st);
+}
+
+struct Carver {
+  char* base;
+  size_t used = 0;
+  explicit Carver(void* p) : base(static_cast<char*>(p)) {}
+  template <typename U>
+  U* take(size_t n) {
+    used = (used + 255) / 256 * 256;
+    U* p = base ? reinterpret_cast<U*>(base + used) : nullptr;
+    used += n * sizeof(U);
+    return p;
+  }
+};
+
+static long long pad_rows(long long rows) { return rows < 1 ? ROW_PAD : (rows + ROW_PAD - 1) / ROW_PAD * ROW_PAD; }
+static int pad_width(int width) { return (width + 7) / 8 * 8; }
+
+struct FwdWs {
+  uint16_t* packed;
+  int32_t* origin;
+  float2* part;
+  float* q;
+  float* cw;
+  int32_t* idx;
+  int32_t* live;
+  size_t bytes;
+};
+static FwdWs fwd_ws(void* ws, int rows, int vocab, int width, int k) {
+  Carver c(ws);
+  FwdWs w;
+  w.packed = c.take<uint16_t>((size_t)pad_rows(rows) * pad_width(width));
+  w.origin = c.take<int32_t>(rows);
+  w.part = c.take<float2>((size_t)2 * ((vocab + BN - 1) / BN) * pad_rows(rows));
+  w.q = c.take<float>((size_t)rows * k);
+  w.cw = c.take<float>((size_t)rows * k);
+  w.idx = c.take<int32_t>((size_t)rows * k);
+  w.live = c.take<int32_t>(k ? rows : 0);
+  w.bytes = c.used + 256;
+  return w;
+}
+
+// Classes per piece of the backward pass: the piece's dz takes 2 bytes per row and class; at most PIECE_BYTES, but not so few classes that
+// the products become short (4096).  Pieces are of nearly equal size.
+constexpr long long PIECE_BYTES = 512ll << 20;
+static int piece_classes(int rows, int vocab) {
+  long long most = PIECE_BYTES / (2 * pad_rows(rows));
+  most = most < 4096 ? 4096 : most;
+  const long long whole = (vocab + BN - 1) / BN;
+  const long long most_tiles = most / BN;
+  const long long pieces = (whole + most_tiles - 1) / most_tiles;
+  return (int)((whole + pieces - 1) / pieces * BN);
+}
+
+struct BwdWs {
+  uint16_t* packed;
+  int32_t* origin;
+  float* lse2;
+  uint16_t* dz;
+  float* acc;
+  int piece;
+  size_t bytes;
+};
+static BwdWs bwd_ws(void* ws, int rows, int vocab, int width) {
+  Carver c(ws);
+  BwdWs w;
+  w.piece = piece_classes(rows, vocab);
+  w.packed = c.take<uint16_t>((size_t)pad_rows(rows) * pad_width(width));
+  w.origin = c.take<int32_t>(rows);
+  w.lse2 = c.take<float>(pad_rows(rows));
+  w.dz = c.take<uint16_t>((size_t)pad_rows(rows) * w.piece);
+  w.acc = c.take<float>(w.piece < vocab ? (size_t)pad_rows(rows) * width : 0);
+  w.bytes = c.used + 256;
+  return w;
+}
+
+static int check_head(const char* fn, const void* hidden, long long ldh, const void* weight, long long ldw, int rows, int vocab, int width,
+                      int dtype, const int32_t* status) {
+  LANCET_REQUIRE(dtype == LANCET_BF16 || dtype == LANCET_F16, LANCET_ERR_UNSUPPORTED,
+                 "%s: hidden rows and weight must be bfloat16 or float16 (dtype code %d)", fn, dtype);
+  LANCET_REQUIRE(rows >= 0 && rows <= (1 << 26) && vocab >= 1 && vocab <= (1 << 26) && width >= 1 && width <= (1 << 20), LANCET_ERR_INVALID,
+                 "%s: bad sizes rows=%d vocab=%d width=%d", fn, rows, vocab, width);
+  LANCET_REQUIRE(ldh >= width && ldw >= width, LANCET_ERR_INVALID, "%s: row strides %lld / %lld below the width %d", fn, ldh, ldw, width);
+  LANCET_REQUIRE(weight && status && (rows == 0 || hidden), LANCET_ERR_NULL, "%s: null pointer argument", fn);
+  LANCET_REQUIRE(aligned(weight, 16) && ldw % 8 == 0, LANCET_ERR_INVALID,
+                 "%s: the weight's rows must start on 16-byte boundaries (row stride %lld)", fn, ldw);
+  LANCET_REQUIRE(aligned(hidden, 2), LANCET_ERR_INVALID, "%s: hidden is not aligned to its type", fn);
+  return LANCET_OK;
+}
+static int check_teacher(const char* fn, int k, float temperature) {
+  LANCET_REQUIRE(k >= 1 && k <= kMaxTop, LANCET_ERR_INVALID, "%s: k=%d top entries (1 to %d)", fn, k, kMaxTop);
+  LANCET_REQUIRE(temperature >= 1e-3f && temperature <= 1e3f, LANCET_ERR_INVALID, "%s: temperature %g outside [0.001, 1000]", fn,
+                 (double)temperature);
+  return LANCET_OK;
+}
+
+struct FwdArgs {
+  const void* hidden;
+  long long ldh;
+  const void* weight;
+  long long ldw;
+  const long long* target;
+  const void* values;
+  int vdtype;
+  const long long* indices;
+  int k;
+  float inv_t;
+  int rows, vocab, width, dtype;
+  float *loss_rows, *lse_rows, *diff;
+  int32_t* pos;
+  float *mean, *inv_live;
+  void* ws;
+  size_t ws_bytes;
+  int32_t* status;
+};
+
+template <typename T>
+static int finish_launch(const FwdArgs& a, const FwdWs& w, int n_part, cudaStream_t st) {
+  const T* packed = reinterpret_cast<const T*>(w.packed);
+  const T* weight = static_cast<const T*>(a.weight);
+  auto go = [&](auto kernel, int rows_per_block) {
+    launch_chained(kernel, dim3((a.rows + rows_per_block - 1) / rows_per_block), dim3(kFinishThreads), 0, st,
+                   static_cast<const float2*>(w.part), pad_rows(a.rows), n_part, static_cast<const int32_t*>(a.pos + a.rows),
+                   static_cast<const int32_t*>(w.origin), packed, pad_width(a.width), weight, a.ldw, a.width, a.target,
+                   static_cast<const int32_t*>(w.idx), static_cast<const float*>(w.q), static_cast<const float*>(w.cw), a.k, a.inv_t,
+                   a.loss_rows, a.lse_rows, a.diff);
+    return launch_status("finish_rows_kernel");
+  };
+  // 32 rows a block read the partial sums in whole lines; with few rows, more blocks
+  if (a.rows >= 2048) return go(finish_rows_kernel<T, 32>, 32);
+  if (a.rows >= 256) return go(finish_rows_kernel<T, 8>, 8);
+  return go(finish_rows_kernel<T, 1>, 1);
+}
+
+static int linear_fwd(const char* fn, const FwdArgs& a, cudaStream_t st) {
+  if (a.rows == 0) return launch_mean(nullptr, nullptr, nullptr, 0, a.mean, a.inv_live, st);
+  const FwdWs w = fwd_ws(a.ws, a.rows, a.vocab, a.width, a.target ? 0 : a.k);
+  LANCET_REQUIRE(a.ws && aligned(a.ws, 256) && a.ws_bytes >= w.bytes, LANCET_ERR_INVALID,
+                 "%s: workspace missing, not aligned to 256 bytes or smaller than %zu bytes", fn, w.bytes);
+  if (!a.target) {
+    launch_chained(teacher_kernel, dim3((a.rows + kTeacherWarps - 1) / kTeacherWarps), dim3(32 * kTeacherWarps), 0, st, a.values, a.vdtype,
+                   a.indices, a.rows, a.k, a.inv_t, a.vocab, w.q, w.cw, w.idx, w.live);
+    if (int rc = launch_status("teacher_kernel")) return rc;
+  }
+  int blocks = (a.rows + 7) / 8;
+  blocks = blocks > 4 * 148 ? 4 * 148 : blocks;
+  launch_chained(pack_rows_kernel, dim3(blocks), dim3(kRowThreads), 0, st, static_cast<const uint16_t*>(a.hidden), a.ldh, a.target,
+                 static_cast<const int32_t*>(a.target ? nullptr : w.live), a.rows, a.vocab, a.width, w.packed, pad_width(a.width), w.origin,
+                 a.pos, a.loss_rows, a.lse_rows);
+  if (int rc = launch_status("pack_rows_kernel")) return rc;
+  const bool paired = paired_for(a.rows);
+  CUtensorMap tmA, tmB;
+  if (int rc = make_map(&tmA, w.packed, pad_rows(a.rows), a.width, pad_width(a.width), BM, a.dtype)) return rc;
+  if (int rc = make_map(&tmB, a.weight, a.vocab, a.width, a.ldw, paired ? BN / 2 : BN, a.dtype)) return rc;
+  Params p = {};
+  p.count = a.pos + a.rows;
+  p.classes = a.vocab;
+  p.width = a.width;
+  p.status = a.status;
+  p.c = a.inv_t * kLog2e;
+  p.part = w.part;
+  p.part_ld = pad_rows(a.rows);
+  int rc = a.dtype == LANCET_BF16 ? launch_product<__nv_bfloat16, FORM_Z, EPI_LSE>(tmA, tmB, p, a.rows, a.vocab, paired, st)
+                                  : launch_product<__half, FORM_Z, EPI_LSE>(tmA, tmB, p, a.rows, a.vocab, paired, st);
+  if (rc) return rc;
+  const int n_part = 2 * ((a.vocab + BN - 1) / BN);
+  rc = a.dtype == LANCET_BF16 ? finish_launch<__nv_bfloat16>(a, w, n_part, st) : finish_launch<__half>(a, w, n_part, st);
+  if (rc) return rc;
+  return launch_mean(a.loss_rows, nullptr, a.pos + a.rows, a.rows, a.mean, a.inv_live, st);
+}
+
+struct BwdArgs {
+  const void* hidden;
+  long long ldh;
+  const void* weight;
+  long long ldw;
+  const long long* target;
+  const float* loss_rows;
+  const long long* indices;
+  const float* diff;
+  int k;
+  float inv_t;
+  const float* lse_rows;
+  const int32_t* pos;
+  int rows, vocab, weight_rows, width, dtype;
+  const float* grad_out;
+  const float* inv_live;
+  float scale;
+  void *dhidden, *dweight;
+  void* ws;
+  size_t ws_bytes;
+  int32_t* status;
+};
+
+template <typename T>
+static int linear_bwd_t(const BwdArgs& a, const BwdWs& w, cudaStream_t st) {
+  int blocks = (a.rows + 7) / 8;
+  blocks = blocks > 4 * 148 ? 4 * 148 : blocks;
+  launch_chained(repack_rows_kernel, dim3(blocks), dim3(kRowThreads), 0, st, static_cast<const uint16_t*>(a.hidden), a.ldh, a.pos, a.lse_rows,
+                 a.rows, a.width, w.packed, pad_width(a.width), w.origin, w.lse2, static_cast<uint16_t*>(a.dhidden));
+  if (int rc = launch_status("repack_rows_kernel")) return rc;
+  const bool paired = paired_for(a.rows);
+  const long long padded = pad_rows(a.rows);
+  // dz is kept in 16 bits.  In float16 it carries a factor of 2^14 (its values are within [-1, 1]): probabilities down to 2^-38 keep their
+  // 11 bits instead of vanishing below 2^-24; the factor leaves again in the products' float32 results.
+  const float shift = a.dtype == LANCET_F16 ? 14.f : 0.f;
+  const float unit = a.dtype == LANCET_F16 ? 16384.f : 1.f;
+  Params p = {};
+  p.count = a.pos + a.rows;
+  p.width = a.width;
+  p.status = a.status;
+  p.c = a.inv_t * kLog2e;
+  p.lse2 = w.lse2;
+  p.shift = shift;
+  p.dz = w.dz;
+  p.dz_ld = w.piece;
+  p.grad_out = a.grad_out;
+  p.inv_live = a.inv_live;
+  p.scale = a.scale / (a.inv_t * unit);
+  CUtensorMap hK, wK, dzK, wMN, dzMN, hMN;
+  if (int rc = make_map(&hK, w.packed, padded, a.width, pad_width(a.width), BM, a.dtype)) return rc;
+  if (int rc = make_map(&wK, a.weight, a.vocab, a.width, a.ldw, paired ? BN / 2 : BN, a.dtype)) return rc;
+  if (int rc = make_map(&dzK, w.dz, padded, w.piece, w.piece, BM, a.dtype)) return rc;
+  if (int rc = make_map(&wMN, a.weight, a.vocab, a.width, a.ldw, 64, a.dtype)) return rc;
+  if (int rc = make_map(&dzMN, w.dz, padded, w.piece, w.piece, 64, a.dtype)) return rc;
+  if (int rc = make_map(&hMN, w.packed, padded, a.width, pad_width(a.width), 64, a.dtype)) return rc;
+  for (int v0 = 0; v0 < a.vocab; v0 += w.piece) {
+    const int classes = a.vocab - v0 < w.piece ? a.vocab - v0 : w.piece;
+    const bool last = v0 + classes == a.vocab;
+    p.class0 = v0;
+    p.classes = classes;
+    if (int rc = launch_product<T, FORM_Z, EPI_PROB>(hK, wK, p, a.rows, classes, paired, st)) return rc;
+    const long long entries = (long long)a.rows * a.k;
+    launch_chained(place_targets_kernel<T>, dim3((unsigned)((entries + 255) / 256)), dim3(256), 0, st, static_cast<const int32_t*>(p.count),
+                   static_cast<const int32_t*>(w.origin), a.target, a.loss_rows, a.indices, a.diff, a.k, v0, classes, unit,
+                   reinterpret_cast<T*>(w.dz), (long long)w.piece);
+    if (int rc = launch_status("place_targets_kernel")) return rc;
+    Params ph = p;
+    ph.out = a.dhidden;
+    ph.row_map = w.origin;
+    if (w.piece < a.vocab) {
+      ph.acc = w.acc;
+      ph.acc_in = v0 > 0;
+      ph.acc_out = !last;
+    }
+    if (a.dhidden)
+      if (int rc = launch_product<T, FORM_DH, EPI_OUT>(dzK, wMN, ph, a.rows, a.width, paired, st)) return rc;
+    if (!a.dweight) continue;
+    Params pw = p;
+    pw.out = a.dweight;
+    if (int rc = launch_product<T, FORM_DW, EPI_OUT>(dzMN, hMN, pw, classes, a.width, paired_for(classes), st)) return rc;
+  }
+  return LANCET_OK;
+}
+
+static int linear_bwd(const char* fn, const BwdArgs& a, cudaStream_t st) {
+  LANCET_REQUIRE(a.weight_rows >= a.vocab, LANCET_ERR_INVALID, "%s: %d weight rows for %d classes", fn, a.weight_rows, a.vocab);
+  LANCET_REQUIRE(a.rows == 0 || (a.lse_rows && a.pos), LANCET_ERR_NULL, "%s: null pointer argument", fn);
+  LANCET_REQUIRE(aligned(a.dhidden, 2) && aligned(a.dweight, 2), LANCET_ERR_INVALID, "%s: outputs are not aligned to their type", fn);
+  uint16_t* dw = static_cast<uint16_t*>(a.dweight);
+  const int first = a.rows == 0 ? 0 : a.vocab;   // rows behind the vocabulary have no gradient
+  if (dw && first < a.weight_rows)
+    LANCET_CUDA(cudaMemsetAsync(dw + (size_t)first * a.width, 0, (size_t)(a.weight_rows - first) * a.width * 2, st));
+  if (a.rows == 0 || (!a.dhidden && !a.dweight)) return LANCET_OK;
+  const BwdWs w = bwd_ws(a.ws, a.rows, a.vocab, a.width);
+  LANCET_REQUIRE(a.ws && aligned(a.ws, 256) && a.ws_bytes >= w.bytes, LANCET_ERR_INVALID,
+                 "%s: workspace missing, not aligned to 256 bytes or smaller than %zu bytes", fn, w.bytes);
+  return a.dtype == LANCET_BF16 ? linear_bwd_t<__nv_bfloat16>(a, w, st) : linear_bwd_t<__half>(a, w, st);
+}
+
+}  // namespace head
+}  // namespace lancet
+
+extern "C" {
+using namespace lancet;
+
+size_t lancet_linear_loss_fwd_workspace_bytes(int rows, int vocab, int width, int k) {
+  if (rows < 0 || vocab < 1 || width < 1 || k < 0) return 0;
+  return head::fwd_ws(nullptr, rows, vocab, width, k).bytes;
+}
+size_t lancet_linear_loss_bwd_workspace_bytes(int rows, int vocab, int width) {
+  if (rows < 0 || vocab < 1 || width < 1) return 0;
+  return head::bwd_ws(nullptr, rows, vocab, width).bytes;
+}
+
+int lancet_linear_xent_fwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, int rows, int vocab,
+                           int width, int dtype, float* loss_rows, float* lse_rows, int32_t* pos, float* mean, float* inv_live, void* ws, size_t ws_bytes,
+                           int32_t* status, lancet_stream_t stream) {
+  const char* fn = "lancet_linear_xent_fwd";
+  if (int rc = head::check_head(fn, hidden, ldh, weight, ldw, rows, vocab, width, dtype, status)) return rc;
+  LANCET_REQUIRE(mean && inv_live && (rows == 0 || (target && loss_rows && lse_rows && pos)), LANCET_ERR_NULL, "%s: null pointer argument", fn);
+  const head::FwdArgs a = {hidden, ldh, weight, ldw, target, nullptr, 0, nullptr, 1, 1.f, rows, vocab, width, dtype, loss_rows, lse_rows,
+                           nullptr, pos, mean, inv_live, ws, ws_bytes, status};
+  return head::linear_fwd(fn, a, static_cast<cudaStream_t>(stream));
+}
+
+int lancet_linear_xent_bwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target,
+                           const float* loss_rows, const float* lse_rows, const int32_t* pos, int rows, int vocab, int weight_rows, int width,
+                           int dtype, const float* grad_out, const float* inv_live, float scale, void* dhidden, void* dweight, void* ws,
+                           size_t ws_bytes, int32_t* status, lancet_stream_t stream) {
+  const char* fn = "lancet_linear_xent_bwd";
+  if (int rc = head::check_head(fn, hidden, ldh, weight, ldw, rows, vocab, width, dtype, status)) return rc;
+  LANCET_REQUIRE(rows == 0 || (target && loss_rows), LANCET_ERR_NULL, "%s: null pointer argument", fn);
+  const head::BwdArgs a = {hidden, ldh, weight, ldw, target, loss_rows, nullptr, nullptr, 1, 1.f, lse_rows, pos, rows, vocab, weight_rows,
+                           width, dtype, grad_out, inv_live, scale, dhidden, dweight, ws, ws_bytes, status};
+  return head::linear_bwd(fn, a, static_cast<cudaStream_t>(stream));
+}
+
+int lancet_linear_distill_fwd(const void* hidden, long long ldh, const void* weight, long long ldw, const void* top_values, int values_dtype,
+                              const long long* top_indices, int k, float temperature, int rows, int vocab, int width, int dtype,
+                              float* loss_rows, float* lse_rows, float* diff, int32_t* pos, float* mean, float* inv_live, void* ws, size_t ws_bytes,
+                              int32_t* status, lancet_stream_t stream) {
+  const char* fn = "lancet_linear_distill_fwd";
+  if (int rc = head::check_head(fn, hidden, ldh, weight, ldw, rows, vocab, width, dtype, status)) return rc;
+  if (int rc = head::check_teacher(fn, k, temperature)) return rc;
+  LANCET_REQUIRE(valid_dtype(values_dtype), LANCET_ERR_INVALID, "%s: unknown dtype code %d of the values", fn, values_dtype);
+  LANCET_REQUIRE(mean && inv_live && (rows == 0 || (top_values && top_indices && loss_rows && lse_rows && diff && pos)), LANCET_ERR_NULL,
+                 "%s: null pointer argument", fn);
+  const head::FwdArgs a = {hidden, ldh, weight, ldw, nullptr, top_values, values_dtype, top_indices, k, 1.0f / temperature, rows, vocab, width,
+                           dtype, loss_rows, lse_rows, diff, pos, mean, inv_live, ws, ws_bytes, status};
+  return head::linear_fwd(fn, a, static_cast<cudaStream_t>(stream));
+}
+
+int lancet_linear_distill_bwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* top_indices,
+                              const float* diff, int k, float temperature, const float* lse_rows, const int32_t* pos, int rows, int vocab,
+                              int weight_rows, int width, int dtype, const float* grad_out, const float* inv_live, float scale, void* dhidden,
+                              void* dweight, void* ws, size_t ws_bytes, int32_t* status, lancet_stream_t stream) {
+  const char* fn = "lancet_linear_distill_bwd";
+  if (int rc = head::check_head(fn, hidden, ldh, weight, ldw, rows, vocab, width, dtype, status)) return rc;
+  if (int rc = head::check_teacher(fn, k, temperature)) return rc;
+  LANCET_REQUIRE(rows == 0 || (top_indices && diff), LANCET_ERR_NULL, "%s: null pointer argument", fn);
+  const head::BwdArgs a = {hidden, ldh, weight, ldw, nullptr, nullptr, top_indices, diff, k, 1.0f / temperature, lse_rows, pos, rows, vocab,
+                           weight_rows, width, dtype, grad_out, inv_live, scale, dhidden, dweight, ws, ws_bytes, status};
+  return head::linear_bwd(fn, a, static_cast<cudaStream_t>(stream));
+}
+}

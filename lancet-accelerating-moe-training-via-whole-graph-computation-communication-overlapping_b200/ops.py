@@ -10,6 +10,7 @@ torch supplies device memory and the current stream only; all arithmetic runs in
 library behind the C ABI.  Extra keyword arguments (k, gates dtype) extend the surface to the
 top-2 gate; their defaults reproduce the reference ops.
 """
+import contextlib
 import ctypes
 
 import torch
@@ -341,6 +342,219 @@ def softmax_xent_bwd(logits, target, vocab, lse, grad_out, scale):
     check(_capi.lib().lancet_softmax_xent_bwd(_ptr(logits), logits.stride(0), _ptr(target), rows, vocab, cols, _dt(logits), _ptr(lse),
                                               _ptr(grad_out) if grad_out is not None else None, float(scale), _ptr(dx),
                                               dx.stride(0), _stream(logits)))
+    return dx
+
+
+def _on(t):
+    """The tensor's device as the current one, where it is not."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _matrix(name, what, t, like=None):
+    """A [rows, cols] CUDA matrix with adjacent columns (copied where they are not) and its row stride."""
+    if not t.is_cuda:
+        raise ValueError("lancet_b200 ops need CUDA tensors (there is no CPU path)")
+    if t.dim() != 2:
+        raise ValueError("%s: %s must be a matrix" % (name, what))
+    if like is not None and t.device != like.device:
+        raise ValueError("%s: %s is on %s, the first operand on %s" % (name, what, t.device, like.device))
+    rows, cols = t.shape
+    if rows > 1 and t.stride(0) < cols or cols > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, max(t.stride(0), cols)
+
+
+def _classes(name, vocab, most):
+    vocab = most if vocab is None else int(vocab)
+    if not 1 <= vocab <= most:
+        raise ValueError("%s: vocab=%d for %d classes" % (name, vocab, most))
+    return vocab
+
+
+def _target_rows(name, target, like):
+    if not target.is_cuda or target.device != like.device or target.dtype != torch.int64 or target.shape != (like.shape[0],):
+        raise TypeError("%s: target must be an int64 vector with an entry per row, on the operands' device" % name)
+    return target.contiguous()
+
+
+def _teacher_rows(name, top_values, top_indices, like):
+    for t in (top_values, top_indices):
+        if not t.is_cuda or t.device != like.device or t.dim() != 2 or t.shape[0] != like.shape[0] or t.shape != top_indices.shape:
+            raise ValueError("%s: the teacher's values and indices must be [rows, k] on the operands' device" % name)
+    if top_indices.dtype != torch.int64:
+        raise TypeError("%s: top_indices must be int64" % name)
+    _dt(top_values)
+    return top_values.contiguous(), top_indices.contiguous()
+
+
+def _head_operands(name, hidden, weight):
+    """hidden [rows, width] and weight [classes, width] as the head's products read them: (hidden, its row stride, weight, its row
+    stride).  A weight whose rows do not start on 16-byte boundaries is copied to a padded row stride."""
+    hidden, ldh = _matrix(name, "hidden", hidden)
+    weight, ldw = _matrix(name, "weight", weight, hidden)
+    if hidden.dtype != weight.dtype or hidden.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("%s: bfloat16 or float16 operands of one type" % name)
+    if weight.shape[1] != hidden.shape[1] or hidden.shape[1] < 1 or weight.shape[0] < 1:
+        raise ValueError("%s: hidden [rows, width] and weight [classes, width] do not match: %s, %s"
+                         % (name, tuple(hidden.shape), tuple(weight.shape)))
+    if ldw % 8 or weight.data_ptr() % 16:
+        ldw = (weight.shape[1] + 7) // 8 * 8
+        padded = torch.empty((weight.shape[0], ldw), dtype=weight.dtype, device=weight.device)
+        padded[:, :weight.shape[1]] = weight
+        weight = padded
+    return hidden, ldh, weight, ldw
+
+
+def _head_status(device):
+    """The status word of the bounded waits (`gemm_status`).  A word first made under stream capture would be filled by the replay
+    only: such a call gets one of its own."""
+    if device not in _gemm_status and torch.cuda.is_current_stream_capturing():
+        return torch.zeros(1, dtype=torch.int32, device=device)
+    return gemm_status(device)
+
+
+def _grad_scalar(name, t, like):
+    if t is not None and (t.dtype != torch.float32 or t.numel() != 1 or t.device != like.device):
+        raise TypeError("%s: grad_out and inv_live must be float32 scalars on the operands' device" % name)
+    return _ptr(t)
+
+
+def _row_floats(like, *shape):
+    return torch.empty(shape, dtype=torch.float32, device=like.device)
+
+
+def linear_xent_fwd(hidden, weight, target, vocab=None):
+    """Cross entropy of the logits `hidden @ weight[:vocab].T` against `target` int64 [rows] (negative or >= vocab: row ignored) without
+    keeping the logits.  hidden [rows, width] and weight [classes, width] bfloat16 or float16.  Returns (loss_rows, lse_rows, mean,
+    inv_live, pos): row losses and log-sum-exp (0 in ignored rows), the mean over the other rows, 1 / their number, and the int32 row list
+    that `linear_xent_bwd` takes.  The workspace is allocated per call: calls on other streams and captured graphs share nothing.  As with
+    the grouped GEMM a wait that ran out is recorded in `gemm_status`."""
+    name = "linear_xent_fwd"
+    hidden, ldh, w, ldw = _head_operands(name, hidden, weight)
+    vocab = _classes(name, vocab, weight.shape[0])
+    target = _target_rows(name, target, hidden)
+    rows, width = hidden.shape
+    loss, lse, mean, inv_live = (_row_floats(hidden, *s) for s in ((rows,), (rows,), (), ()))
+    pos = torch.empty((rows + 1,), dtype=torch.int32, device=hidden.device)
+    L = _capi.lib()
+    with _on(hidden):
+        nws = L.lancet_linear_loss_fwd_workspace_bytes(rows, vocab, width, 0)
+        ws = torch.empty(nws, dtype=torch.uint8, device=hidden.device)
+        check(L.lancet_linear_xent_fwd(_ptr(hidden), ldh, _ptr(w), ldw, _ptr(target), rows, vocab, width, _dt(hidden), _ptr(loss), _ptr(lse),
+                                       _ptr(pos), _ptr(mean), _ptr(inv_live), _ptr(ws), nws, _ptr(_head_status(hidden.device)),
+                                       _stream(hidden)))
+    return loss, lse, mean, inv_live, pos
+
+
+def linear_xent_bwd(hidden, weight, target, loss_rows, lse_rows, pos, vocab=None, grad_out=None, inv_live=None, scale=1.0,
+                    need_hidden=True, need_weight=True):
+    """Gradients (dhidden, dweight) of sum(loss_rows) * grad_out * inv_live * scale for `linear_xent_fwd`, in the operands' type; what is
+    not needed is None.  grad_out and inv_live: float32 scalars on the device, or None for 1.  Weight rows from `vocab` on and
+    hidden rows of ignored rows get zeros."""
+    name = "linear_xent_bwd"
+    hidden, ldh, w, ldw = _head_operands(name, hidden, weight)
+    vocab = _classes(name, vocab, weight.shape[0])
+    target = _target_rows(name, target, hidden)
+    _require_cuda(loss_rows, lse_rows, pos)
+    rows, width = hidden.shape
+    if loss_rows.shape != (rows,) or lse_rows.shape != (rows,) or pos.shape != (rows + 1,):
+        raise ValueError("%s: loss_rows, lse_rows and pos must be those of the forward call" % name)
+    dh = torch.empty((rows, width), dtype=hidden.dtype, device=hidden.device) if need_hidden else None
+    dw = torch.empty(tuple(weight.shape), dtype=weight.dtype, device=weight.device) if need_weight else None
+    L = _capi.lib()
+    with _on(hidden):
+        nws = L.lancet_linear_loss_bwd_workspace_bytes(rows, vocab, width)
+        ws = torch.empty(nws, dtype=torch.uint8, device=hidden.device)
+        check(L.lancet_linear_xent_bwd(_ptr(hidden), ldh, _ptr(w), ldw, _ptr(target), _ptr(loss_rows), _ptr(lse_rows), _ptr(pos), rows, vocab,
+                                       weight.shape[0], width, _dt(hidden), _grad_scalar(name, grad_out, hidden),
+                                       _grad_scalar(name, inv_live, hidden), float(scale), _ptr(dh), _ptr(dw), _ptr(ws), nws,
+                                       _ptr(_head_status(hidden.device)), _stream(hidden)))
+    return dh, dw
+
+
+def linear_distill_fwd(hidden, weight, top_values, top_indices, temperature=1.0, vocab=None):
+    """Distillation loss of the logits `hidden @ weight[:vocab].T` against a teacher's top logits, without keeping the logits: with
+    q = softmax(top_values / T) over the row's entries, loss_rows = T^2 sum q (log q - log softmax(logits / T)[top_indices]).
+    top_values [rows, k] float32, float16 or bfloat16, top_indices [rows, k] int64, k <= 512; an index that names no class does not
+    count (NaN in its value included), a row without counting entries is ignored.  Returns (loss_rows, lse_rows, mean, inv_live, pos, diff)
+    as `linear_xent_fwd` does; diff [rows, k] float32 is the student's minus the teacher's probability at the entries."""
+    name = "linear_distill_fwd"
+    hidden, ldh, w, ldw = _head_operands(name, hidden, weight)
+    vocab = _classes(name, vocab, weight.shape[0])
+    top_values, top_indices = _teacher_rows(name, top_values, top_indices, hidden)
+    (rows, width), k = hidden.shape, top_indices.shape[1]
+    loss, lse, mean, inv_live, diff = (_row_floats(hidden, *s) for s in ((rows,), (rows,), (), (), (rows, k)))
+    pos = torch.empty((rows + 1,), dtype=torch.int32, device=hidden.device)
+    L = _capi.lib()
+    with _on(hidden):
+        nws = L.lancet_linear_loss_fwd_workspace_bytes(rows, vocab, width, k)
+        ws = torch.empty(nws, dtype=torch.uint8, device=hidden.device)
+        check(L.lancet_linear_distill_fwd(_ptr(hidden), ldh, _ptr(w), ldw, _ptr(top_values), _dt(top_values), _ptr(top_indices), k,
+                                          float(temperature), rows, vocab, width, _dt(hidden), _ptr(loss), _ptr(lse), _ptr(diff), _ptr(pos),
+                                          _ptr(mean), _ptr(inv_live), _ptr(ws), nws, _ptr(_head_status(hidden.device)), _stream(hidden)))
+    return loss, lse, mean, inv_live, pos, diff
+
+
+def linear_distill_bwd(hidden, weight, top_indices, diff, lse_rows, pos, temperature=1.0, vocab=None, grad_out=None, inv_live=None,
+                       scale=1.0, need_hidden=True, need_weight=True):
+    """Gradients (dhidden, dweight) of `linear_distill_fwd`, as `linear_xent_bwd` gives them."""
+    name = "linear_distill_bwd"
+    hidden, ldh, w, ldw = _head_operands(name, hidden, weight)
+    vocab = _classes(name, vocab, weight.shape[0])
+    _, top_indices = _teacher_rows(name, diff, top_indices, hidden)
+    _require_cuda(diff, lse_rows, pos)
+    (rows, width), k = hidden.shape, top_indices.shape[1]
+    if diff.dtype != torch.float32 or lse_rows.shape != (rows,) or pos.shape != (rows + 1,):
+        raise ValueError("%s: diff, lse_rows and pos must be those of the forward call" % name)
+    dh = torch.empty((rows, width), dtype=hidden.dtype, device=hidden.device) if need_hidden else None
+    dw = torch.empty(tuple(weight.shape), dtype=weight.dtype, device=weight.device) if need_weight else None
+    L = _capi.lib()
+    with _on(hidden):
+        nws = L.lancet_linear_loss_bwd_workspace_bytes(rows, vocab, width)
+        ws = torch.empty(nws, dtype=torch.uint8, device=hidden.device)
+        check(L.lancet_linear_distill_bwd(_ptr(hidden), ldh, _ptr(w), ldw, _ptr(top_indices), _ptr(diff), k, float(temperature), _ptr(lse_rows),
+                                          _ptr(pos), rows, vocab, weight.shape[0], width, _dt(hidden), _grad_scalar(name, grad_out, hidden),
+                                          _grad_scalar(name, inv_live, hidden), float(scale), _ptr(dh), _ptr(dw), _ptr(ws), nws,
+                                          _ptr(_head_status(hidden.device)), _stream(hidden)))
+    return dh, dw
+
+
+def distill_fwd(logits, top_values, top_indices, temperature=1.0, vocab=None):
+    """The loss of `linear_distill_fwd` on given logits [rows, cols] (float32, float16 or bfloat16; columns from `vocab` on are padding
+    and never read).  Returns (loss_rows, lse_rows, mean, inv_live, live_rows, class_weights); the last two are kept for `distill_bwd`."""
+    name = "distill_fwd"
+    logits, ld = _matrix(name, "logits", logits)
+    dt = _dt(logits)
+    vocab = _classes(name, vocab, logits.shape[1])
+    top_values, top_indices = _teacher_rows(name, top_values, top_indices, logits)
+    rows, k = logits.shape[0], top_indices.shape[1]
+    loss, lse, mean, inv_live, weights = (_row_floats(logits, *s) for s in ((rows,), (rows,), (), (), (rows, k)))
+    live = torch.empty((rows,), dtype=torch.int32, device=logits.device)
+    with _on(logits):
+        check(_capi.lib().lancet_distill_fwd(_ptr(logits), ld, _ptr(top_values), _dt(top_values), _ptr(top_indices), k, float(temperature),
+                                             rows, vocab, dt, _ptr(loss), _ptr(lse), _ptr(weights), _ptr(live), _ptr(mean), _ptr(inv_live),
+                                             _stream(logits)))
+    return loss, lse, mean, inv_live, live, weights
+
+
+def distill_bwd(logits, top_indices, class_weights, live_rows, lse_rows, temperature=1.0, vocab=None, grad_out=None, inv_live=None,
+                scale=1.0):
+    """Gradient of sum(loss_rows) * grad_out * inv_live * scale with respect to the logits, in their type and shape; padded columns and
+    ignored rows are zero."""
+    name = "distill_bwd"
+    logits, ld = _matrix(name, "logits", logits)
+    dt = _dt(logits)
+    vocab = _classes(name, vocab, logits.shape[1])
+    _, top_indices = _teacher_rows(name, class_weights, top_indices, logits)
+    _require_cuda(class_weights, live_rows, lse_rows)
+    (rows, cols), k = logits.shape, top_indices.shape[1]
+    if class_weights.dtype != torch.float32 or lse_rows.shape != (rows,) or live_rows.shape != (rows,):
+        raise ValueError("%s: class_weights, live_rows and lse_rows must be those of the forward call" % name)
+    dx = torch.empty((rows, cols), dtype=logits.dtype, device=logits.device)
+    with _on(logits):
+        check(_capi.lib().lancet_distill_bwd(_ptr(logits), ld, _ptr(top_indices), _ptr(class_weights), _ptr(live_rows), k, float(temperature),
+                                             rows, vocab, cols, dt, _ptr(lse_rows), _grad_scalar(name, grad_out, logits),
+                                             _grad_scalar(name, inv_live, logits), float(scale), _ptr(dx), cols, _stream(logits)))
     return dx
 
 

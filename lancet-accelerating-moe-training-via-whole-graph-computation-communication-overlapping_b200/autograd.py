@@ -291,58 +291,50 @@ def softmax_cross_entropy(logits, target, vocab=None):
     return _SoftmaxCrossEntropy.apply(logits, target, logits.shape[1] if vocab is None else vocab)
 
 
-class _LinearCrossEntropy(torch.autograd.Function):
+class _LinearLoss(torch.autograd.Function):
+    """The linear losses: a target per row (k = 0), or a teacher's values and indices.  What the forward pass leaves for the backward one is
+    one buffer; operands are saved as the kernels read them and not checked again."""
+
     @staticmethod
-    def forward(ctx, hidden, weight, target, vocab):
-        loss_rows, lse, mean, inv_live, pos = ops.linear_xent_fwd(hidden, weight, target, vocab)
-        ctx.save_for_backward(hidden, weight, target, loss_rows, lse, pos, inv_live)
-        ctx.vocab = vocab
+    def forward(ctx, name, hidden, weight, vocab, target, teacher, temperature):
+        mean, state, h, w, target, ctx.vocab = ops._linear_fwd(name, hidden, weight, vocab, target, teacher, temperature)
+        ctx.save_for_backward(h, w, target, state)
+        ctx.name, ctx.classes, ctx.k = name, weight.shape[0], 0 if teacher is None else target.shape[1]
+        ctx.temperature = float(temperature)
         return mean
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        hidden, weight, target, loss_rows, lse, pos, inv_live = ctx.saved_tensors
-        dh, dw = ops.linear_xent_bwd(hidden, weight, target, loss_rows, lse, pos, ctx.vocab, gout, inv_live,
-                                     need_hidden=ctx.needs_input_grad[0], need_weight=ctx.needs_input_grad[1])
-        return dh, dw, None, None
-
-
-class _LinearDistillation(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, hidden, weight, top_values, top_indices, temperature, vocab):
-        _, lse, mean, inv_live, pos, diff = ops.linear_distill_fwd(hidden, weight, top_values, top_indices, temperature, vocab)
-        ctx.save_for_backward(hidden, weight, top_indices, lse, pos, diff, inv_live)
-        ctx.temperature, ctx.vocab = temperature, vocab
-        return mean
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gout):
-        hidden, weight, top_indices, lse, pos, diff, inv_live = ctx.saved_tensors
-        dh, dw = ops.linear_distill_bwd(hidden, weight, top_indices, diff, lse, pos, ctx.temperature, ctx.vocab, gout, inv_live,
-                                        need_hidden=ctx.needs_input_grad[0], need_weight=ctx.needs_input_grad[1])
-        return dh, dw, None, None, None, None
+        h, w, target, state = ctx.saved_tensors
+        loss, lse, inv_live, pos, diff = ops._state_ptrs(state, h.shape[0])
+        dh, dw = ops._linear_bwd(ctx.name, h, max(h.stride(0), h.shape[1]), w, max(w.stride(0), w.shape[1]), ctx.classes, ctx.vocab, target,
+                                 loss, lse, pos, diff if ctx.k else None, ctx.k, ctx.temperature, gout.data_ptr(), inv_live, 1.0,
+                                 ctx.needs_input_grad[1], ctx.needs_input_grad[2])
+        return None, dh, dw, None, None, None, None
 
 
 class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_values, top_indices, temperature, vocab):
-        _, lse, mean, inv_live, live, weights = ops.distill_fwd(logits, top_values, top_indices, temperature, vocab)
-        ctx.save_for_backward(logits, top_indices, weights, live, lse, inv_live)
-        ctx.temperature, ctx.vocab = temperature, vocab
+        mean, state, x, indices, ctx.vocab = ops._distill_fwd(logits, top_values, top_indices, temperature, vocab)
+        ctx.save_for_backward(x, indices, state)
+        ctx.temperature = float(temperature)
         return mean
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        logits, top_indices, weights, live, lse, inv_live = ctx.saved_tensors
-        return ops.distill_bwd(logits, top_indices, weights, live, lse, ctx.temperature, ctx.vocab, gout, inv_live), None, None, None, None
+        x, indices, state = ctx.saved_tensors
+        _, lse, inv_live, live, weights = ops._state_ptrs(state, x.shape[0])
+        return ops._distill_bwd(x, max(x.stride(0), x.shape[1]), indices, ctx.vocab, weights, live, lse, ctx.temperature, gout.data_ptr(),
+                                inv_live, 1.0), None, None, None, None
 
 
 def _head_inputs(hidden, weight):
     """Rows of the head as F.linear would see them: any leading axes, the autocast type inside an autocast region."""
-    hidden = hidden.reshape(-1, hidden.shape[-1])
+    if hidden.dim() != 2:
+        hidden = hidden.reshape(-1, hidden.shape[-1])
     if hidden.is_cuda and torch.is_autocast_enabled("cuda"):
         dt = torch.get_autocast_dtype("cuda")
         hidden, weight = hidden.to(dt), weight.to(dt)
@@ -356,7 +348,7 @@ def linear_cross_entropy(hidden, weight, target, vocab=None):
     [...] int64 (negative or >= vocab = ignored), weight rows from `vocab` on are padding.  The sums are float32; the gradient of the logits
     passes between the products in the operands' type, as it does between a loss and F.linear."""
     hidden, weight = _head_inputs(hidden, weight)
-    return _LinearCrossEntropy.apply(hidden, weight, target.reshape(-1), vocab)
+    return _LinearLoss.apply("linear_cross_entropy", hidden, weight, vocab, target.reshape(-1), None, 1.0)
 
 
 def linear_distillation_loss(hidden, weight, top_values, top_indices, temperature=1.0, vocab=None):
@@ -364,7 +356,8 @@ def linear_distillation_loss(hidden, weight, top_values, top_indices, temperatur
     `linear_cross_entropy`, top_values and top_indices [..., k]."""
     hidden, weight = _head_inputs(hidden, weight)
     k = top_indices.shape[-1]
-    return _LinearDistillation.apply(hidden, weight, top_values.detach().reshape(-1, k), top_indices.reshape(-1, k), temperature, vocab)
+    return _LinearLoss.apply("linear_distillation_loss", hidden, weight, vocab, None,
+                             (top_values.detach().reshape(-1, k), top_indices.reshape(-1, k)), temperature)
 
 
 def distillation_loss(logits, top_values, top_indices, temperature=1.0, vocab=None):

@@ -100,18 +100,45 @@ __device__ __forceinline__ void merge(float& m, float& s, float m2, float s2, fl
   m = mm;
 }
 
+// A row is read by one block, or with few rows by the blocks of a cluster: contiguous shares of its 16-byte vectors, the maxima and sums
+// joined through the cluster's shared memory in rank order.
+struct Share {
+  int v0, v1;         // vectors of this block
+  bool first, last;   // has the elements before the first vector, behind the last one
+};
+__device__ __forceinline__ Share share_of(int nv, int part, int parts) {
+  Share s;
+  s.v0 = (int)((long long)nv * part / parts);
+  s.v1 = (int)((long long)nv * (part + 1) / parts);
+  s.first = part == 0;
+  s.last = part == parts - 1;
+  return s;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float cluster_load(const float* p, int rank) {
+  uint32_t local = (uint32_t)__cvta_generic_to_shared(p), remote;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  return v;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 distill_fwd_kernel(const T* __restrict__ x, long long ld, const void* __restrict__ values, int vdtype, const long long* __restrict__ indices,
-                   int k, float inv_t, int V, float* __restrict__ loss, float* __restrict__ lse, float* __restrict__ weights,
+                   int k, float inv_t, int V, int parts, float* __restrict__ loss, float* __restrict__ lse, float* __restrict__ weights,
                    int32_t* __restrict__ live_rows) {
   chain_enter();
   constexpr int N = Vec<T>::N;
   __shared__ float s_q[kMaxTop];
   __shared__ int s_idx[kMaxTop];
   __shared__ float s_m[kThreads / 32], s_s[kThreads / 32];
+  __shared__ float s_part[2];
   __shared__ int s_live;
-  const long long r = blockIdx.x;
+  const int part = blockIdx.x % parts;   // rank in the row's cluster
+  const long long r = blockIdx.x / parts;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float c = inv_t * kLog2e;
   if (warp == 0) {
@@ -119,9 +146,10 @@ distill_fwd_kernel(const T* __restrict__ x, long long ld, const void* __restrict
     if (lane == 0) s_live = live;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < k; i += kThreads) weights[r * k + i] = class_weight(s_q, s_idx, k, i);
-  if (!s_live) {
-    if (threadIdx.x == 0) {
+  if (part == 0)
+    for (int i = threadIdx.x; i < k; i += kThreads) weights[r * k + i] = class_weight(s_q, s_idx, k, i);
+  if (!s_live) {   // in all blocks of the cluster alike
+    if (part == 0 && threadIdx.x == 0) {
       loss[r] = 0.f;
       lse[r] = 0.f;
       live_rows[r] = 0;
@@ -131,19 +159,21 @@ distill_fwd_kernel(const T* __restrict__ x, long long ld, const void* __restrict
   const T* row = x + r * ld;
   float m = -FLT_MAX, s = 0.f;
   const int head = row_head(row, V);
-  if ((int)threadIdx.x < head) add_one(m, s, Num<T>::to_f(row[threadIdx.x]), c);
   const int nv = (V - head) / N;
+  const Share sh = share_of(nv, part, parts);
   const Vec<T>* rv = reinterpret_cast<const Vec<T>*>(row + head);
-  int i = threadIdx.x;
-  for (; i + 3 * kThreads < nv; i += 4 * kThreads) {   // four loads in flight
+  if (sh.first && (int)threadIdx.x < head) add_one(m, s, Num<T>::to_f(row[threadIdx.x]), c);
+  int i = sh.v0 + threadIdx.x;
+  for (; i + 3 * kThreads < sh.v1; i += 4 * kThreads) {   // four loads in flight
     const Vec<T> a = rv[i], b = rv[i + kThreads], d = rv[i + 2 * kThreads], e = rv[i + 3 * kThreads];
     add_vec(m, s, a, c);
     add_vec(m, s, b, c);
     add_vec(m, s, d, c);
     add_vec(m, s, e, c);
   }
-  for (; i < nv; i += kThreads) add_vec(m, s, rv[i], c);
-  for (int j = head + nv * N + threadIdx.x; j < V; j += kThreads) add_one(m, s, Num<T>::to_f(row[j]), c);
+  for (; i < sh.v1; i += kThreads) add_vec(m, s, rv[i], c);
+  if (sh.last)
+    for (int j = head + nv * N + threadIdx.x; j < V; j += kThreads) add_one(m, s, Num<T>::to_f(row[j]), c);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, m, d), s2 = __shfl_xor_sync(0xffffffffu, s, d);
@@ -154,9 +184,19 @@ distill_fwd_kernel(const T* __restrict__ x, long long ld, const void* __restrict
     s_s[warp] = s;
   }
   __syncthreads();
-  if (warp == 0) {
-    float M = s_m[0], S = s_s[0];
-    for (int w = 1; w < kThreads / 32; ++w) merge(M, S, s_m[w], s_s[w], c);
+  float M = s_m[0], S = s_s[0];
+  for (int w = 1; w < kThreads / 32; ++w) merge(M, S, s_m[w], s_s[w], c);
+  if (parts > 1) {
+    if (threadIdx.x == 0) {
+      s_part[0] = M;
+      s_part[1] = S;
+    }
+    cluster_barrier();
+    if (part == 0 && warp == 0)
+      for (int p = 1; p < parts; ++p) merge(M, S, cluster_load(&s_part[0], p), cluster_load(&s_part[1], p), c);
+    cluster_barrier();   // no block leaves while its sums are read
+  }
+  if (part == 0 && warp == 0) {
     const float l = M * inv_t + logf(S);
     float sum = 0.f;
     for (int e = lane; e < k; e += 32)
@@ -174,23 +214,22 @@ distill_fwd_kernel(const T* __restrict__ x, long long ld, const void* __restrict
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 distill_bwd_kernel(const T* __restrict__ x, long long ld, const long long* __restrict__ indices, const float* __restrict__ weights,
-                   const int32_t* __restrict__ live_rows, int k, float inv_t, int V, int cols, const float* __restrict__ lse,
+                   const int32_t* __restrict__ live_rows, int k, float inv_t, int V, int cols, int parts, const float* __restrict__ lse,
                    const float* __restrict__ gout, const float* __restrict__ inv_live, float scale, T* __restrict__ dx, long long ldd) {
   chain_enter();
   constexpr int N = Vec<T>::N;
-  const long long r = blockIdx.x;
+  const int part = blockIdx.x % parts;
+  const long long r = blockIdx.x / parts;
   const T* row = x + r * ld;
   T* drow = dx + r * ldd;
-  if (!live_rows[r]) {
-    for (int j = threadIdx.x; j < cols; j += kThreads) drow[j] = Num<T>::from_f(0.f);
-    return;
-  }
+  const bool live = live_rows[r] != 0;
   const float g = scale * (gout ? *gout : 1.f) * (inv_live ? *inv_live : 1.f) / inv_t;
   const float c = inv_t * kLog2e, l = lse[r] / inv_t;   // differences of raw values, as in the forward pass
-  // vectors where both rows meet 16-byte boundaries at the same element
+  // vectors where both rows meet 16-byte boundaries at the same element; the blocks of a row take contiguous shares of them
   const bool same = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(drow)) & 15) == 0;
-  const int head = same ? row_head(row, V) : V;
-  const int nv = (V - head) / N;
+  const int head = same ? row_head(row, V) : 0;
+  const int nv = same ? (V - head) / N : 0;
+  const Share sh = share_of(nv, part, parts);
   const Vec<T>* rv = reinterpret_cast<const Vec<T>*>(row + head);
   Vec<T>* dv = reinterpret_cast<Vec<T>*>(drow + head);
   auto grad = [&](float v) { return Num<T>::from_f(ex2f((v - l) * c) * g); };
@@ -200,40 +239,81 @@ distill_bwd_kernel(const T* __restrict__ x, long long ld, const long long* __res
     for (int j = 0; j < N; ++j) o.v[j] = grad(Num<T>::to_f(a.v[j]));
     return o;
   };
-  for (int j = threadIdx.x; j < head; j += kThreads) drow[j] = grad(Num<T>::to_f(row[j]));
-  int i = threadIdx.x;
-  for (; i + 3 * kThreads < nv; i += 4 * kThreads) {
+  // single elements: those outside the vectors, or without vectors this block's share of the row
+  const int tail0 = head + nv * N;
+  const Share single = share_of(cols - tail0, same ? 0 : part, same ? 1 : parts);
+  auto one = [&](int j) { drow[j] = live && j < V ? grad(Num<T>::to_f(row[j])) : Num<T>::from_f(0.f); };
+  if (sh.first && (int)threadIdx.x < head) one(threadIdx.x);
+  if (sh.last || !same)
+    for (int j = tail0 + single.v0 + threadIdx.x; j < tail0 + single.v1; j += kThreads) one(j);
+  if (!live) {
+    Vec<T> z;
+#pragma unroll
+    for (int j = 0; j < N; ++j) z.v[j] = Num<T>::from_f(0.f);
+    for (int i = sh.v0 + threadIdx.x; i < sh.v1; i += kThreads) dv[i] = z;
+    return;
+  }
+  int i = sh.v0 + threadIdx.x;
+  for (; i + 3 * kThreads < sh.v1; i += 4 * kThreads) {
     const Vec<T> a0 = rv[i], a1 = rv[i + kThreads], a2 = rv[i + 2 * kThreads], a3 = rv[i + 3 * kThreads];
     dv[i] = grad_vec(a0);
     dv[i + kThreads] = grad_vec(a1);
     dv[i + 2 * kThreads] = grad_vec(a2);
     dv[i + 3 * kThreads] = grad_vec(a3);
   }
-  for (; i < nv; i += kThreads) dv[i] = grad_vec(rv[i]);
-  for (int j = head + nv * N + threadIdx.x; j < cols; j += kThreads) drow[j] = j < V ? grad(Num<T>::to_f(row[j])) : Num<T>::from_f(0.f);
+  for (; i < sh.v1; i += kThreads) dv[i] = grad_vec(rv[i]);
   __syncthreads();
-  // the teacher's classes: difference in float32, rounded once (entries of one class write the same value)
+  // the teacher's classes, each by the block that wrote its element: difference in float32, rounded once (entries of one class write the same
+  // value)
+  const int from = same ? (sh.first ? 0 : head + sh.v0 * N) : single.v0;
+  const int to = same ? (sh.last ? V : head + sh.v1 * N) : single.v1;
   for (int e = threadIdx.x; e < k; e += kThreads) {
     const long long at = indices[r * k + e];
-    if (at >= 0 && at < V) drow[at] = Num<T>::from_f((ex2f((Num<T>::to_f(row[at]) - l) * c) - weights[r * k + e]) * g);
+    if (at >= from && at < to && at < V) drow[at] = Num<T>::from_f((ex2f((Num<T>::to_f(row[at]) - l) * c) - weights[r * k + e]) * g);
   }
+}
+
+// Blocks per row: one is enough to fill the GPU from four blocks per SM on; a share is at least 16 KB of vectors.
+static int parts_for(int rows, int vocab, int bytes) {
+  int parts = 1;
+  while (parts < 8 && 2ll * parts * rows <= 4 * sm_count() && (long long)vocab * bytes / (2 * parts) >= 16384) parts *= 2;
+  return parts;
+}
+// A chained launch, in clusters of `parts` blocks where the kernel joins its blocks' sums.
+template <typename... KArgs, typename... Args>
+static int launch_rows(void (*kernel)(KArgs...), const char* name, int rows, int parts, bool cluster, cudaStream_t st, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)rows * parts);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = chained_launch_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = parts;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster && parts > 1 ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+  return launch_status(name);
 }
 
 template <typename T>
 static int fwd_t(const void* x, long long ld, const void* values, int vdtype, const long long* indices, int k, float inv_t, int rows, int vocab,
                  float* loss, float* lse, float* weights, int32_t* live_rows, cudaStream_t st) {
-  launch_chained(distill_fwd_kernel<T>, dim3(rows), dim3(kThreads), 0, st, static_cast<const T*>(x), ld, values, vdtype, indices, k, inv_t,
-                 vocab, loss, lse, weights, live_rows);
-  return launch_status("distill_fwd_kernel");
+  const int parts = parts_for(rows, vocab, sizeof(T));
+  return launch_rows(distill_fwd_kernel<T>, "distill_fwd_kernel", rows, parts, true, st, static_cast<const T*>(x), ld, values, vdtype, indices,
+                     k, inv_t, vocab, parts, loss, lse, weights, live_rows);
 }
 
 template <typename T>
 static int bwd_t(const void* x, long long ld, const long long* indices, const float* weights, const int32_t* live_rows, int k, float inv_t,
                  int rows, int vocab, int cols, const float* lse, const float* gout, const float* inv_live, float scale, void* dx,
                  long long ldd, cudaStream_t st) {
-  launch_chained(distill_bwd_kernel<T>, dim3(rows), dim3(kThreads), 0, st, static_cast<const T*>(x), ld, indices, weights, live_rows, k,
-                 inv_t, vocab, cols, lse, gout, inv_live, scale, static_cast<T*>(dx), ldd);
-  return launch_status("distill_bwd_kernel");
+  const int parts = parts_for(rows, vocab, sizeof(T));
+  return launch_rows(distill_bwd_kernel<T>, "distill_bwd_kernel", rows, parts, false, st, static_cast<const T*>(x), ld, indices, weights,
+                     live_rows, k, inv_t, vocab, cols, parts, lse, gout, inv_live, scale, static_cast<T*>(dx), ldd);
 }
 
 }  // namespace head

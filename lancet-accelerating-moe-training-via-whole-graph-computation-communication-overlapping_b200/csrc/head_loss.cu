@@ -7,8 +7,7 @@
 // the vocabulary in pieces: the same product again with an epilogue that writes exp(z / T - lse) of the piece in 16 bits, a small kernel
 // that puts the differences at the targets in place, and two products from that piece.  2 + 2 + 4 flops per row, class and width element.
 //
-// Rows without a target (or teacher) take no part: a first kernel packs the live rows together (dense rows, zeros up to the next tile
-// boundary), every product works on their number, which stays on the device, and the gradient rows go back through the row list.  So an
+// Rows without a target (or teacher) take no part: a first kernel packs the live rows together (dense rows), every product works on their number, which stays on the device, and the gradient rows go back through the row list.  So an
 // ignored row may hold anything, NaN included, and costs a copy's time only.
 //
 // All products run on one kernel: tcgen05.mma from 128-byte-swizzled tiles staged by TMA, float32 accumulators in TMEM, two of them so that
@@ -26,7 +25,7 @@ constexpr int A_STAGE_BYTES = BM * BK * 2;
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int TMEM_COLS = 512;
-constexpr int ROW_PAD = 256;                    // packed rows are padded with zeros to a multiple of this
+constexpr int ROW_PAD = 256;                    // row buffers hold a multiple of this: whole tiles, in the paired form too
 constexpr long long BAND_BYTES = 20ll << 20;    // rows of A swept against all columns before the next band: they stay in L2
 
 // Products (A's and B's rows are M and N):
@@ -56,6 +55,8 @@ struct Params {
   // EPI_LSE: per (column half tile, row) maximum and sum in the base-2 domain
   float2* part;
   long long part_ld;
+  const int32_t* tgt;     // target of every packed row, or null; its logit goes to zt
+  float* zt;
   // EPI_PROB: 2^(z c - lse2[row] + shift) of the piece
   const float* lse2;
   float shift;
@@ -69,6 +70,7 @@ struct Params {
   float scale;
   float* acc;               // float32 sums over the pieces, or null
   int acc_in, acc_out;      // add the sums so far / store sums instead of the output
+  float* slots;             // partial sums of split tiles
 };
 
 struct Dims {
@@ -89,14 +91,75 @@ __device__ __forceinline__ Dims dims_of(const Params& p) {
   return d;
 }
 
+// A reduction over classes or rows is long where the tiles are few.  The workers first take whole tiles in turn as long as each gets one;
+// what is left (`rem` tiles) is cut along the reduction into equal contiguous ranges, a range per worker, so that all of them end together.
+// A range spans two tiles at most; parts of a tile go to float32 slots (2 per worker) and are added in order by join_tiles_kernel.
+// Cutting pays when the idle share of the last turn costs more than the join ((workers - rem) / workers x kb blocks of 512 clocks against
+// about 8000 clocks) and is more than a quarter of all turns: below that the GPU, which runs these products at its power limit, clocks higher
+// while some SMs idle, and the parts' traffic costs more than the turn (8192 rows x 1024, 128 tiles on 74 pairs: 2.67 ms for the
+// step with whole tiles, 2.77 cut).
+constexpr int SPLIT_MIN_KB = 16;
+constexpr int SPLIT_MIN_PART = 4;
+struct Split {
+  int full, rem, parts, kb;   // whole tiles, tiles that are cut, ranges they are cut into, blocks of a tile
+  long long iters;
+  __host__ __device__ long long begin(int w) const { return iters * w / parts; }
+};
+__host__ __device__ __forceinline__ Split split_of(int n_tiles, int kb, int workers) {
+  Split s = {n_tiles, 0, 1, kb, 0};
+  const int rem = n_tiles % workers;
+  const long long idle = workers - rem, turns = (n_tiles + workers - 1) / workers;
+  if (rem > 0 && idle * kb > (long long)SPLIT_MIN_KB * workers && 4 * idle > turns * workers) {
+    s.full = n_tiles - rem;
+    s.rem = rem;
+    s.iters = (long long)rem * kb;
+    long long parts = s.iters / SPLIT_MIN_PART;
+    parts = parts < rem ? rem : parts;
+    s.parts = (int)(parts > workers ? workers : parts);
+  }
+  return s;
+}
+// The items of one worker: a tile, the blocks [k0, k1) of its reduction, and the slot of a partial sum (-1: the whole tile).
+struct Walk {
+  Split s;
+  int worker, workers, next;
+  long long pos, end, first;
+  int t, k0, k1, slot;
+  __device__ __forceinline__ Walk(int n_tiles, int kb, int w, int n, bool may_split) : worker(w), workers(n), next(w) {
+    s = may_split ? split_of(n_tiles, kb, n) : Split{n_tiles, 0, 1, kb, 0};
+    pos = end = first = 0;
+    if (s.rem > 0 && w < s.parts) {
+      first = pos = s.begin(w);
+      end = s.begin(w + 1);
+    }
+  }
+  __device__ __forceinline__ bool step() {
+    if (next < s.full) {
+      t = next;
+      next += workers;
+      k0 = 0;
+      k1 = s.kb;
+      slot = -1;
+      return true;
+    }
+    if (pos >= end) return false;
+    const int j = (int)(pos / s.kb);
+    k0 = (int)(pos - (long long)j * s.kb);
+    k1 = (int)min((long long)s.kb, k0 + end - pos);
+    t = s.full + j;
+    slot = k0 == 0 && k1 == s.kb ? -1 : 2 * worker + (pos == first ? 0 : 1);
+    pos += k1 - k0;
+    return true;
+  }
+};
+
 struct Tile {
   int mt, nt;   // this CTA's 128-row tile, column tile
 };
 // FORM_Z: bands of row units that stay in L2, swept against the column tiles.  Otherwise the index with fewer tiles runs fastest: the tiles
 // in flight form a block as square as possible and share the most operand slabs.
 template <int FORM, bool CTA2>
-__device__ __forceinline__ Tile decode(const Params& p, const Dims& d, int t, int rank) {
-  int mu, nt;
+__device__ __forceinline__ void decode_unit(const Params& p, const Dims& d, int t, int& mu, int& nt) {
   if (FORM == FORM_Z) {
     const long long unit_bytes = (long long)(CTA2 ? 2 * BM : BM) * p.width * 2;
     int band = (int)(BAND_BYTES / unit_bytes);
@@ -113,6 +176,11 @@ __device__ __forceinline__ Tile decode(const Params& p, const Dims& d, int t, in
     nt = t / d.mu;
     mu = t - nt * d.mu;
   }
+}
+template <int FORM, bool CTA2>
+__device__ __forceinline__ Tile decode(const Params& p, const Dims& d, int t, int rank) {
+  int mu, nt;
+  decode_unit<FORM, CTA2>(p, d, t, mu, nt);
   Tile tl;
   tl.mt = CTA2 ? 2 * mu + rank : mu;
   tl.nt = nt;
@@ -132,7 +200,8 @@ __device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-template <typename T, int FORM, int EPI, bool CTA2>
+// ACC (EPI_OUT): sums over the pieces pass through p.acc
+template <typename T, int FORM, int EPI, bool CTA2, bool ACC>
 __global__ void __launch_bounds__(THREADS, 1)
 head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, Params p) {
   using C = Cfg<CTA2>;
@@ -182,7 +251,7 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const uint32_t tmem_base = *tmem_slot;
   chain_enter();                  // the set-up above overlaps the previous kernel's end; its results are read from here on
   const Dims d = dims_of<FORM, CTA2>(p);
-  const int n_tiles = d.mu * d.nt;
+  Walk walk(d.mu * d.nt, d.kb, worker, n_workers, EPI == EPI_OUT);
 
   if (warp == 0) {
     // ---------------- TMA producer (one per CTA; in the paired form each CTA loads its own halves) ----------------
@@ -191,10 +260,10 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       uint32_t phase = 0;
       bool ok = true;
       const int b_off = CTA2 ? rank * (BN / 2) : 0;   // this CTA's share of the tile's columns
-      for (int t = worker; t < n_tiles && ok; t += n_workers) {
-        const Tile tl = decode<FORM, CTA2>(p, d, t, rank);
+      while (ok && walk.step()) {
+        const Tile tl = decode<FORM, CTA2>(p, d, walk.t, rank);
         const int m0 = tl.mt * BM, n0 = tl.nt * BN + b_off;
-        for (int kb = 0; kb < d.kb; ++kb) {
+        for (int kb = walk.k0; kb < walk.k1; ++kb) {
           if (!(ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.status, 11))) break;
           const uint32_t a_dst = smem_u32(sA + stage * A_STAGE_BYTES), b_dst = smem_u32(sB + stage * C::B_STAGE_BYTES);
           uint32_t full = bar_full + 8 * stage;
@@ -227,13 +296,13 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       int stage = 0;
       uint32_t phase = 0;
       int buf = 0;
-      uint32_t tphase[2] = {0, 0};
+      uint32_t tphase = 0;
       bool ok = true;
-      for (int t = worker; t < n_tiles && ok; t += n_workers) {
-        if (!(ok = mbar_wait(bar_tempty + 8 * buf, tphase[buf] ^ 1, abort_flag, p.status, 12))) break;
+      while (ok && walk.step()) {
+        if (!(ok = mbar_wait(bar_tempty + 8 * buf, ((tphase >> buf) & 1) ^ 1, abort_flag, p.status, 12))) break;
         tc_fence_after();
         const uint32_t tmem_d = tmem_base + (uint32_t)(buf * BN);
-        for (int kb = 0; kb < d.kb; ++kb) {
+        for (int kb = walk.k0; kb < walk.k1; ++kb) {
           if (!(ok = mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, 13))) break;
           tc_fence_after();
           const uint32_t a_addr = smem_u32(sA + stage * A_STAGE_BYTES);
@@ -243,16 +312,16 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             const uint64_t adesc = A_MN ? smem_desc_mn_sw128(a_addr + k * 2048) : smem_desc_k_sw128(a_addr + k * UMMA_K * 2);
             const uint64_t bdesc = B_MN ? smem_desc_mn_sw128(b_addr + k * 2048) : smem_desc_k_sw128(b_addr + k * UMMA_K * 2);
             if (CTA2)
-              umma_f16_pair(tmem_d, adesc, bdesc, idesc, (kb | k) ? 1u : 0u);
+              umma_f16_pair(tmem_d, adesc, bdesc, idesc, (kb > walk.k0 || k) ? 1u : 0u);
             else
-              umma_f16(tmem_d, adesc, bdesc, idesc, (kb | k) ? 1u : 0u);
+              umma_f16(tmem_d, adesc, bdesc, idesc, (kb > walk.k0 || k) ? 1u : 0u);
           }
           if (CTA2) umma_commit_pair(bar_empty + 8 * stage); else umma_commit(bar_empty + 8 * stage);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
         if (!ok) break;
         if (CTA2) umma_commit_pair(bar_tfull + 8 * buf); else umma_commit(bar_tfull + 8 * buf);
-        tphase[buf] ^= 1;
+        tphase ^= 1u << buf;
         buf ^= 1;
       }
     }
@@ -261,25 +330,92 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const int quad = warp & 3, half = (warp - 2) >> 2;
     constexpr int CHUNKS = BN / 64;   // 32-column chunks of a half tile
     int buf = 0;
-    uint32_t tphase[2] = {0, 0};
+    uint32_t tphase = 0;
     bool ok = true;
     float g = 1.f;
     if (EPI == EPI_OUT) g = p.scale * (p.grad_out ? *p.grad_out : 1.f) * (p.inv_live ? *p.inv_live : 1.f);
+    auto release = [&]() {   // the accumulator may be overwritten once every epilogue warp (of both CTAs) has read it
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (CTA2) mbar_arrive_cluster(cluster_addr(bar_tempty + 8 * buf, 0)); else mbar_arrive(bar_tempty + 8 * buf);
+      }
+      tphase ^= 1u << buf;
+      buf ^= 1;
+    };
+    const bool vec = p.width % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
     const uint32_t acc_mask = d.kb > 0 ? 0xffffffffu : 0u;   // no live rows: the accumulator holds stale values
-    for (int t = worker; t < n_tiles && ok; t += n_workers) {
-      const Tile tl = decode<FORM, CTA2>(p, d, t, rank);
+    while (ok && walk.step()) {
+      const Tile tl = decode<FORM, CTA2>(p, d, walk.t, rank);
       const int row = tl.mt * BM + quad * 32 + lane;
       const bool row_live = row < d.m;
       const int col_first = tl.nt * BN + half * (BN / 2);
       float off = 0.f;
       long long out_row = row;
       if (EPI == EPI_PROB && row_live) off = p.shift - p.lse2[row];
-      if (EPI == EPI_OUT && row_live) out_row = p.row_map ? (p.acc_out ? row : p.row_map[row]) : (long long)p.class0 + row;
-      ok = mbar_wait(bar_tfull + 8 * buf, tphase[buf], abort_flag, p.status, 14);
+      if (EPI == EPI_OUT && row_live) out_row = p.row_map ? p.row_map[row] : (long long)p.class0 + row;
+      ok = mbar_wait(bar_tfull + 8 * buf, (tphase >> buf) & 1, abort_flag, p.status, 14);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN + half * (BN / 2));
+      if (EPI == EPI_OUT && walk.slot >= 0) {
+        float* dst = p.slots + ((long long)walk.slot * (CTA2 ? 2 * BM : BM) + rank * BM + quad * 32 + lane) * BN + half * (BN / 2);
+#pragma unroll 1
+        for (int ch = 0; ch < CHUNKS; ++ch) {
+          uint32_t r[32];
+          tmem_ld32(taddr + ch * 32, r);
+          if (row_live) {
+#pragma unroll
+            for (int q = 0; q < 32; q += 8)
+              st_global_32B(dst + ch * 32 + q, make_uint4(r[q], r[q + 1], r[q + 2], r[q + 3]),
+                            make_uint4(r[q + 4], r[q + 5], r[q + 6], r[q + 7]));
+          }
+        }
+        release();
+        continue;
+      }
+      if (EPI == EPI_OUT) {
+        // whole chunks of rows on 32-byte boundaries first: one loop without other control flow around the TMEM loads and the stores
+        const int left = d.n - col_first;
+        const int whole = ACC || !vec ? 0 : min(CHUNKS, left / 32);
+        T* dst = static_cast<T*>(p.out) + out_row * p.width + col_first;
+#pragma unroll 1
+        for (int ch = 0; ch < whole; ++ch) {
+          uint32_t r[32], o[16];
+          tmem_ld32(taddr + ch * 32, r);
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            o[i >> 1] = pack_pair<T>(__uint_as_float(r[i] & acc_mask) * g, __uint_as_float(r[i + 1] & acc_mask) * g);
+          if (row_live) {
+#pragma unroll
+            for (int q = 0; q < 4; q += 2)
+              st_global_32B(dst + ch * 32 + 8 * q, make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]),
+                            make_uint4(o[4 * q + 4], o[4 * q + 5], o[4 * q + 6], o[4 * q + 7]));
+          }
+        }
+#pragma unroll 1
+        for (int ch = whole; ch < CHUNKS && ch * 32 < left; ++ch) {
+          uint32_t r[32];
+          tmem_ld32(taddr + ch * 32, r);
+          if (!row_live) continue;
+          float* acc = ACC ? p.acc + (long long)row * p.width + col_first + ch * 32 : nullptr;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (ch * 32 + i >= left) continue;
+            float v = __uint_as_float(r[i] & acc_mask);
+            if (ACC && p.acc_in) v += acc[i];
+            if (ACC && p.acc_out)
+              acc[i] = v;
+            else
+              dst[ch * 32 + i] = Num<T>::from_f(v * g);
+          }
+        }
+        release();
+        continue;
+      }
+      int want = -1;               // EPI_LSE: column of the row's target in this half tile
+      if (EPI == EPI_LSE && p.tgt && row_live) want = p.tgt[row] - col_first;
       float m = -1e30f, s = 0.f;   // EPI_LSE: maximum of z and sum of 2^((z - m) c)
 #pragma unroll 1
       for (int ch = 0; ch < CHUNKS; ++ch) {
@@ -320,46 +456,20 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           for (int q = 0; q < 4; q += 2)
             st_global_32B(dst + q, make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]),
                           make_uint4(o[4 * q + 4], o[4 * q + 5], o[4 * q + 6], o[4 * q + 7]));
-        } else if (row_live && left > 0) {
-          float v[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i] & acc_mask);
-          if (p.acc && p.acc_in) {
-            const float* a = p.acc + (long long)row * p.width + col_first + ch * 32;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += i < left ? a[i] : 0.f;
-          }
-          if (p.acc && p.acc_out) {
-            float* a = p.acc + (long long)row * p.width + col_first + ch * 32;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i < left) a[i] = v[i];
-          } else {
-            T* dst = static_cast<T*>(p.out) + out_row * p.width + col_first + ch * 32;
-            if (left >= 32 && (reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
-              uint32_t o[16];
-#pragma unroll
-              for (int i = 0; i < 32; i += 2) o[i >> 1] = pack_pair<T>(v[i] * g, v[i + 1] * g);
-#pragma unroll
-              for (int q = 0; q < 4; q += 2)
-                st_global_32B(dst + 8 * q, make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]),
-                              make_uint4(o[4 * q + 4], o[4 * q + 5], o[4 * q + 6], o[4 * q + 7]));
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (i < left) dst[i] = Num<T>::from_f(v[i] * g);
-            }
-          }
+        }
+      }
+      if (EPI == EPI_LSE) {
+        // the few targets in this half tile: their columns once more
+        unsigned hits = __ballot_sync(0xffffffffu, want >= 0 && want < BN / 2);
+        while (hits) {
+          const int owner = __ffs(hits) - 1, col = __shfl_sync(0xffffffffu, want, owner);
+          const uint32_t z = tmem_ld1(taddr + col);
+          if (lane == owner) p.zt[row] = __uint_as_float(z);
+          hits &= hits - 1;
         }
       }
       if (EPI == EPI_LSE && row_live) p.part[(long long)(2 * tl.nt + half) * p.part_ld + row] = make_float2(m * p.c, s);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (CTA2) mbar_arrive_cluster(cluster_addr(bar_tempty + 8 * buf, 0)); else mbar_arrive(bar_tempty + 8 * buf);
-      }
-      tphase[buf] ^= 1;
-      buf ^= 1;
+      release();
     }
   }
   // ---------------- teardown ----------------
@@ -382,6 +492,86 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
 }
 
+// Adds the parts of split tiles in a fixed order and finishes them as the product's epilogue does.  A block takes JOIN_ROWS rows of a tile, a
+// thread four columns; where a tile has many parts (few rows), the block's four groups of threads share the parts of one row, else each group has
+// a row of its own.
+constexpr int JOIN_ROWS = 4, JOIN_SHARED_PARTS = 8;
+template <typename T, int FORM, bool CTA2>
+__global__ void __launch_bounds__(256) join_tiles_kernel(Params p, int workers) {
+  chain_enter();
+  __shared__ float4 s_part[4][64];
+  const Dims d = dims_of<FORM, CTA2>(p);
+  const Split s = split_of(d.mu * d.nt, d.kb, workers);
+  const int j = blockIdx.x;
+  if (j >= s.rem) return;
+  int mu, nt;
+  decode_unit<FORM, CTA2>(p, d, s.full + j, mu, nt);
+  constexpr int UNIT = CTA2 ? 2 * BM : BM;
+  const int row0 = blockIdx.y * JOIN_ROWS;
+  if (mu * UNIT + row0 >= d.m) return;
+  const long long a = (long long)j * s.kb, b = a + s.kb;
+  int w0 = (int)(a * s.parts / s.iters), w1;
+  while (w0 > 0 && s.begin(w0) > a) --w0;
+  while (s.begin(w0 + 1) <= a) ++w0;
+  w1 = (int)((b - 1) * s.parts / s.iters);   // the worker that has the last block
+  while (w1 > 0 && s.begin(w1) > b - 1) --w1;
+  while (s.begin(w1 + 1) <= b - 1) ++w1;
+  const bool late = s.begin(w0) < a;         // the first worker began in the tile before: this is its second part
+  if (w0 == w1 && !late && s.begin(w0 + 1) == b) return;   // one worker had all of it
+  const float g = p.scale * (p.grad_out ? *p.grad_out : 1.f) * (p.inv_live ? *p.inv_live : 1.f);
+  const int col = (threadIdx.x & 63) * 4, grp = threadIdx.x >> 6;
+  const int n0 = nt * BN + col;
+  auto sum = [&](int i, int from, int step) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int w = from; w <= w1; w += step) {
+      const int slot = 2 * w + (w == w0 && late ? 1 : 0);
+      const float4 x = *reinterpret_cast<const float4*>(p.slots + ((long long)slot * UNIT + i) * BN + col);
+      v.x += x.x;
+      v.y += x.y;
+      v.z += x.z;
+      v.w += x.w;
+    }
+    return v;
+  };
+  auto finish = [&](int i, const float4& x) {
+    const int row = mu * UNIT + i;
+    const float v[4] = {x.x, x.y, x.z, x.w};
+    float* acc = p.acc + (long long)row * p.width + n0;
+    T* out = static_cast<T*>(p.out) + (p.row_map ? p.row_map[row] : (long long)p.class0 + row) * p.width + n0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if (n0 + c >= d.n) break;
+      const float t = p.acc && p.acc_in ? v[c] + acc[c] : v[c];
+      if (p.acc && p.acc_out)
+        acc[c] = t;
+      else
+        out[c] = Num<T>::from_f(t * g);
+    }
+  };
+  if (w1 - w0 < JOIN_SHARED_PARTS) {
+    const int i = row0 + grp;
+    if (mu * UNIT + i < d.m) finish(i, sum(i, w0, 1));
+  } else {
+    for (int i = row0; i < row0 + JOIN_ROWS && mu * UNIT + i < d.m; ++i) {
+      s_part[grp][threadIdx.x & 63] = sum(i, w0 + grp, 4);
+      __syncthreads();
+      if (grp == 0) {
+        float4 v = s_part[0][threadIdx.x];
+        for (int o = 1; o < 4; ++o) {
+          const float4 x = s_part[o][threadIdx.x];
+          v.x += x.x;
+          v.y += x.y;
+          v.z += x.z;
+          v.w += x.w;
+        }
+        finish(i, v);
+      }
+      __syncthreads();
+    }
+  }
+}
+
 // ---- live rows ------------------------------------------------------------------------------------------------------------
 constexpr int kRowThreads = 256;
 
@@ -401,12 +591,12 @@ __device__ __forceinline__ bool row_is_live(const long long* target, const int32
   return t >= 0 && t < vocab;
 }
 
-// Packs the live rows: pos[r] = packed index of row r or -1, pos[rows] = their number, packed rows, zero rows up to the next multiple of
-// ROW_PAD.  Each block owns a range of rows and first counts the live rows before it.
+// Packs the live rows: pos[r] = packed index of row r or -1, pos[rows] = their number, packed rows.  Each block owns a range of rows and first
+// counts the live rows before it.  What the buffer holds behind them reaches only results that no one keeps.
 __global__ void __launch_bounds__(kRowThreads)
 pack_rows_kernel(const uint16_t* __restrict__ hidden, long long ld, const long long* __restrict__ target, const int32_t* __restrict__ flags,
                  int rows, int vocab, int width, uint16_t* __restrict__ packed, int packed_ld, int32_t* __restrict__ origin,
-                 int32_t* __restrict__ pos, float* __restrict__ loss_rows, float* __restrict__ lse_rows) {
+                 int32_t* __restrict__ tgt, int32_t* __restrict__ pos, float* __restrict__ loss_rows, float* __restrict__ lse_rows) {
   chain_enter();
   __shared__ int s_warp[kRowThreads / 32];
   __shared__ int s_at[kRowThreads];
@@ -435,6 +625,7 @@ pack_rows_kernel(const uint16_t* __restrict__ hidden, long long ld, const long l
       pos[r] = live ? at : -1;
       if (live) {
         origin[at] = r;
+        if (target) tgt[at] = (int)target[r];
       } else {
         loss_rows[r] = 0.f;
         lse_rows[r] = 0.f;
@@ -446,14 +637,11 @@ pack_rows_kernel(const uint16_t* __restrict__ hidden, long long ld, const long l
       if (s_at[i] >= 0) copy_row(packed + (long long)s_at[i] * packed_ld, hidden + (long long)(base + i) * ld, width);
     for (int w = 0; w < kRowThreads / 32; ++w) before += s_warp[w];
   }
-  if (blockIdx.x == gridDim.x - 1) {
-    if (threadIdx.x == 0) pos[rows] = before;
-    const int end = (before + ROW_PAD - 1) / ROW_PAD * ROW_PAD;
-    for (int i = before + warp; i < end; i += kRowThreads / 32) copy_row(packed + (long long)i * packed_ld, nullptr, width);
-  }
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) pos[rows] = before;
 }
 
-// The same packing in the backward pass, from pos; gradient rows of ignored rows are zeroed, lse goes to packed order and base 2.
+// The same packing in the backward pass, from pos; gradient rows of ignored rows are zeroed, lse goes to packed order and base 2.  dW sums over
+// blocks of BK rows: the last one is filled up with zeros (dz has zeros there, but 0 x NaN would remain).
 __global__ void __launch_bounds__(kRowThreads)
 repack_rows_kernel(const uint16_t* __restrict__ hidden, long long ld, const int32_t* __restrict__ pos, const float* __restrict__ lse_rows,
                    int rows, int width, uint16_t* __restrict__ packed, int packed_ld, int32_t* __restrict__ origin, float* __restrict__ lse2,
@@ -474,99 +662,147 @@ repack_rows_kernel(const uint16_t* __restrict__ hidden, long long ld, const int3
       copy_row(dhidden + (long long)r * width, nullptr, width);
     }
   }
-  const int count = pos[rows], end = (count + ROW_PAD - 1) / ROW_PAD * ROW_PAD;
+  const int count = pos[rows], end = (count + BK - 1) / BK * BK;
   for (int i = count + first; i < end; i += warps) copy_row(packed + (long long)i * packed_ld, nullptr, width);
 }
 
 // ---- row results ----------------------------------------------------------------------------------------------------------
 constexpr int kFinishThreads = 256;
 
-template <typename T>
-__device__ __forceinline__ float warp_dot(const T* a, const T* b, int width) {
+// N dot products of row a with rows of b by one warp, their loads in flight together.  All rows start on 16-byte boundaries (packed rows; the
+// weight's rows as the tensor map wants them).
+template <typename T, int N>
+__device__ __forceinline__ void warp_dots(const T* a, const T* const* b, int width, float* out) {
   const int lane = threadIdx.x & 31;
-  float s = 0.f;
-  // both rows start on 16-byte boundaries (packed rows; the weight's rows as the tensor map wants them)
+  float s[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) s[n] = 0.f;
   const int nv = width / 8;
+#pragma unroll 2
   for (int i = lane; i < nv; i += 32) {
-    const uint4 x = reinterpret_cast<const uint4*>(a)[i], y = reinterpret_cast<const uint4*>(b)[i];
+    const uint4 x = reinterpret_cast<const uint4*>(a)[i];
+    uint4 y[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) y[n] = __ldg(reinterpret_cast<const uint4*>(b[n]) + i);
     const T* xs = reinterpret_cast<const T*>(&x);
-    const T* ys = reinterpret_cast<const T*>(&y);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s = fmaf(Num<T>::to_f(xs[j]), Num<T>::to_f(ys[j]), s);
+    for (int n = 0; n < N; ++n) {
+      const T* ys = reinterpret_cast<const T*>(&y[n]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[n] = fmaf(Num<T>::to_f(xs[j]), Num<T>::to_f(ys[j]), s[n]);
+    }
   }
-  for (int i = nv * 8 + lane; i < width; i += 32) s = fmaf(Num<T>::to_f(a[i]), Num<T>::to_f(b[i]), s);
+  for (int i = nv * 8 + lane; i < width; i += 32)
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-  return s;
+    for (int n = 0; n < N; ++n) s[n] = fmaf(Num<T>::to_f(a[i]), Num<T>::to_f(b[n][i]), s[n]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1)
+#pragma unroll
+    for (int n = 0; n < N; ++n) s[n] += __shfl_xor_sync(0xffffffffu, s[n], d);
+#pragma unroll
+  for (int n = 0; n < N; ++n) out[n] = s[n];
 }
 
-// A block finishes kRows packed rows: joins the partial maxima and sums of its rows' column half tiles (in tile order), then each warp
-// takes rows and computes the logits at their targets as dot products.  k entries per row: idx [rows][k] (-1: none), q and class weights
-// [rows][k]; or a target per row.
+// A block finishes kRows packed rows: joins the partial maxima and sums of its rows' column half tiles (in a fixed order), then its warps
+// compute the logits at the rows' targets, or at the k entries of their teachers (idx [rows][k], -1: none), as float32 dot products.  The
+// tensor cores cut the sums of products short (measured: up to 1e-5 low at a logit of 12), which the loss would show where a target
+// holds most of the probability: its share of the row's sum is replaced by the dot product's.
 template <typename T, int kRows>
 __global__ void __launch_bounds__(kFinishThreads)
 finish_rows_kernel(const float2* __restrict__ part, long long part_ld, int n_part, const int32_t* __restrict__ count,
                    const int32_t* __restrict__ origin, const T* __restrict__ packed, int packed_ld, const T* __restrict__ weight,
-                   long long weight_ld, int width, const long long* __restrict__ target, const int32_t* __restrict__ idx,
-                   const float* __restrict__ q, const float* __restrict__ cw, int k, float inv_t, float* __restrict__ loss_rows,
-                   float* __restrict__ lse_rows, float* __restrict__ diff) {
+                   long long weight_ld, int width, const int32_t* __restrict__ tgt, const float* __restrict__ zt,
+                   const int32_t* __restrict__ idx, const float* __restrict__ q, const float* __restrict__ cw, int k, float inv_t,
+                   float* __restrict__ loss_rows, float* __restrict__ lse_rows, float* __restrict__ diff) {
   chain_enter();
-  constexpr int G = kFinishThreads / kRows;
-  __shared__ float s_m[G][kRows], s_s[G][kRows];
+  constexpr int G = kFinishThreads / kRows, W = kFinishThreads / 32;
+  constexpr int DOTS = 4;
+  extern __shared__ float s_terms[];   // [kRows][k] terms of the teachers' sums
+  __shared__ float s_m[W][kRows], s_s[W][kRows];
   __shared__ float s_lse[kRows];
   const int n = *count;
   const int base = blockIdx.x * kRows;
   if (base >= n) return;
+  const int live = min(kRows, n - base);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rr = threadIdx.x % kRows, grp = threadIdx.x / kRows;
-  float m = -INFINITY, s = 0.f;
-  if (base + rr < n) {
-    m = -1e38f;
+  float m = -1e38f, s = 0.f;
+  auto merge = [&](float m2, float s2) {
+    const float mm = fmaxf(m, m2);
+    s = s * ex2f(m - mm) + s2 * ex2f(m2 - mm);
+    m = mm;
+  };
+  if (rr < live) {
+#pragma unroll 4
     for (int t = grp; t < n_part; t += G) {
       const float2 v = part[(long long)t * part_ld + base + rr];
-      const float mm = fmaxf(m, v.x);
-      s = s * ex2f(m - mm) + v.y * ex2f(v.x - mm);
-      m = mm;
+      merge(v.x, v.y);
     }
   }
-  s_m[grp][rr] = m;
-  s_s[grp][rr] = s;
-  __syncthreads();
-  if (grp == 0 && base + rr < n) {
-    for (int j = 1; j < G; ++j) {
-      const float m2 = s_m[j][rr], mm = fmaxf(m, m2);
-      s = s * ex2f(m - mm) + s_s[j][rr] * ex2f(m2 - mm);
-      m = mm;
-    }
-    s_lse[rr] = m * kLn2 + logf(s);
+#pragma unroll
+  for (int d = kRows; d < 32; d <<= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, d), s2 = __shfl_xor_sync(0xffffffffu, s, d);
+    merge(m2, s2);
+  }
+  if (lane < kRows) {
+    s_m[warp][lane] = m;
+    s_s[warp][lane] = s;
   }
   __syncthreads();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = warp; i < kRows && base + i < n; i += kFinishThreads / 32) {
-    const int c = base + i;
-    const long long r = origin[c];
-    const float lse = s_lse[i];
-    const T* h = packed + (long long)c * packed_ld;
-    if (target) {
-      const float z = warp_dot(h, weight + target[r] * weight_ld, width);
+  if (threadIdx.x < live) {
+    m = s_m[0][threadIdx.x];
+    s = s_s[0][threadIdx.x];
+    for (int w = 1; w < W; ++w) merge(s_m[w][threadIdx.x], s_s[w][threadIdx.x]);
+    s_lse[threadIdx.x] = m * kLn2 + logf(s);
+  }
+  __syncthreads();
+  if (!idx) {
+    for (int i = warp; i < live; i += W) {
+      const int c = base + i;
+      const T* b[1] = {weight + (long long)tgt[c] * weight_ld};
+      float z;
+      warp_dots<T, 1>(packed + (long long)c * packed_ld, b, width, &z);
       if (lane == 0) {
-        loss_rows[r] = lse - z;
-        lse_rows[r] = lse;
+        const int r = origin[c];
+        const float fixed = s_lse[i] + log1pf(expf(zt[c] - s_lse[i]) * expm1f(z - zt[c]));
+        loss_rows[r] = fixed - z;
+        lse_rows[r] = fixed;
       }
-    } else {
-      float sum = 0.f;
-      for (int e = 0; e < k; ++e) {
-        const long long at = r * k + e;
-        const int cls = idx[at];
-        if (cls < 0) continue;
-        const float lp = warp_dot(h, weight + (long long)cls * weight_ld, width) * inv_t - lse;
-        const float qe = q[at];
-        if (qe != 0.f) sum += qe * (logf(qe) - lp);
-        if (lane == 0) diff[at] = expf(lp) - cw[at];
-      }
-      if (lane == 0) {
-        loss_rows[r] = sum / (inv_t * inv_t);
-        lse_rows[r] = lse;
-      }
+    }
+    return;
+  }
+  const int per_row = (k + DOTS - 1) / DOTS;
+  for (int t = warp; t < live * per_row; t += W) {
+    const int i = t / per_row, e0 = (t - i * per_row) * DOTS, c = base + i;
+    const long long at = (long long)origin[c] * k;
+    const T* b[DOTS];
+    int cls[DOTS];
+#pragma unroll
+    for (int o = 0; o < DOTS; ++o) {
+      cls[o] = e0 + o < k ? idx[at + e0 + o] : -1;
+      b[o] = weight + (long long)(cls[o] < 0 ? 0 : cls[o]) * weight_ld;
+    }
+    float z[DOTS];
+    warp_dots<T, DOTS>(packed + (long long)c * packed_ld, b, width, z);
+    if (lane < DOTS && e0 + lane < k) {
+      const int e = e0 + lane;
+      const float mine = lane == 0 ? z[0] : lane == 1 ? z[1] : lane == 2 ? z[2] : z[3];
+      const int have = lane == 0 ? cls[0] : lane == 1 ? cls[1] : lane == 2 ? cls[2] : cls[3];
+      const float lp = mine * inv_t - s_lse[i], qe = q[at + e];
+      s_terms[i * k + e] = have >= 0 && qe != 0.f ? qe * (logf(qe) - lp) : 0.f;
+      diff[at + e] = have >= 0 ? expf(lp) - cw[at + e] : 0.f;
+    }
+  }
+  __syncthreads();
+  for (int i = warp; i < live; i += W) {
+    float sum = 0.f;
+    for (int e = lane; e < k; e += 32) sum += s_terms[i * k + e];
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) {
+      const int r = origin[base + i];
+      loss_rows[r] = sum / (inv_t * inv_t);
+      lse_rows[r] = s_lse[i];
     }
   }
 }
@@ -627,9 +863,10 @@ static int make_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t 
 // The paired form halves the bytes of B through shared memory per product; up to 128 rows its second tile would be empty.
 static bool paired_for(int m) { return m > BM; }
 
-template <typename T, int FORM, int EPI, bool CTA2>
-static int launch_form(const CUtensorMap& tmA, const CUtensorMap& tmB, const Params& p, long long units, cudaStream_t st) {
-  auto kernel = head_product_kernel<T, FORM, EPI, CTA2>;
+template <typename T, int FORM, int EPI, bool CTA2, bool ACC>
+static int launch_form(const CUtensorMap& tmA, const CUtensorMap& tmB, const Params& p, long long units, bool split, int* workers,
+                       cudaStream_t st) {
+  auto kernel = head_product_kernel<T, FORM, EPI, CTA2, ACC>;
   constexpr int SMEM = Cfg<CTA2>::SMEM_BYTES;
   static int set_for[64] = {0};   // per device
   int dev = 0;
@@ -640,9 +877,10 @@ static int launch_form(const CUtensorMap& tmA, const CUtensorMap& tmB, const Par
   }
   long long grid = sm_count();
   if (gemm_cta_limit() > 0 && gemm_cta_limit() < grid) grid = gemm_cta_limit();
-  if (grid > units * (CTA2 ? 2 : 1)) grid = units * (CTA2 ? 2 : 1);
+  if (!split && grid > units * (CTA2 ? 2 : 1)) grid = units * (CTA2 ? 2 : 1);
   if (CTA2) grid &= ~1ll;
   if (grid < (CTA2 ? 2 : 1)) grid = CTA2 ? 2 : 1;
+  *workers = (int)grid / (CTA2 ? 2 : 1);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(THREADS);
@@ -664,12 +902,37 @@ static int launch_form(const CUtensorMap& tmA, const CUtensorMap& tmB, const Par
   return launch_status("head_product_kernel");
 }
 
-template <typename T, int FORM, int EPI>
-static int launch_product(const CUtensorMap& tmA, const CUtensorMap& tmB, const Params& p, int m, int n, bool paired, cudaStream_t st) {
-  const long long unit = paired ? 2 * BM : BM;
-  const long long units = ((m + unit - 1) / unit) * ((n + BN - 1) / BN);
+template <typename T, int FORM, int EPI, bool CTA2>
+static int launch_product_as(const CUtensorMap& tmA, const CUtensorMap& tmB, const Params& p, int m, int n, int k, cudaStream_t st) {
+  constexpr int UNIT = CTA2 ? 2 * BM : BM;
+  const long long units = ((long long)(m + UNIT - 1) / UNIT) * ((n + BN - 1) / BN);
   LANCET_REQUIRE(units < (1ll << 30), LANCET_ERR_INVALID, "head product: %lld tiles", units);
-  return paired ? launch_form<T, FORM, EPI, true>(tmA, tmB, p, units, st) : launch_form<T, FORM, EPI, false>(tmA, tmB, p, units, st);
+  const bool split = EPI == EPI_OUT && (k + BK - 1) / BK > SPLIT_MIN_KB;   // the least length of a reduction that split_of cuts
+  int workers = 0;
+  if constexpr (FORM == FORM_DH) {
+    if (p.acc) {
+      if (int rc = launch_form<T, FORM, EPI, CTA2, true>(tmA, tmB, p, units, split, &workers, st)) return rc;
+    } else if (int rc = launch_form<T, FORM, EPI, CTA2, false>(tmA, tmB, p, units, split, &workers, st)) {
+      return rc;
+    }
+  } else if (int rc = launch_form<T, FORM, EPI, CTA2, false>(tmA, tmB, p, units, split, &workers, st)) {
+    return rc;
+  }
+  if constexpr (EPI == EPI_OUT) {
+    if (split) {
+      const int most = (int)(units < workers ? units : workers);   // tiles that can have been cut
+      const int rows = m < UNIT ? (m + JOIN_ROWS - 1) / JOIN_ROWS : UNIT / JOIN_ROWS;
+      launch_chained(join_tiles_kernel<T, FORM, CTA2>, dim3(most, rows), dim3(256), 0, st, p, workers);
+      return launch_status("join_tiles_kernel");
+    }
+  }
+  return LANCET_OK;
+}
+// m, n, k: upper bounds of the product's sizes (the live rows are known on the device only)
+template <typename T, int FORM, int EPI>
+static int launch_product(const CUtensorMap& tmA, const CUtensorMap& tmB, const Params& p, int m, int n, int k, bool paired, cudaStream_t st) {
+  return paired ? launch_product_as<T, FORM, EPI, true>(tmA, tmB, p, m, n, k, st)
+                : launch_product_as<T, FORM, EPI, false>(tmA, tmB, p, m, n, k, st);
 }
 
 struct Carver {
@@ -692,6 +955,8 @@ struct FwdWs {
   uint16_t* packed;
   int32_t* origin;
   float2* part;
+  int32_t* tgt;
+  float* zt;
   float* q;
   float* cw;
   int32_t* idx;
@@ -704,6 +969,8 @@ static FwdWs fwd_ws(void* ws, int rows, int vocab, int width, int k) {
   w.packed = c.take<uint16_t>((size_t)pad_rows(rows) * pad_width(width));
   w.origin = c.take<int32_t>(rows);
   w.part = c.take<float2>((size_t)2 * ((vocab + BN - 1) / BN) * pad_rows(rows));
+  w.tgt = c.take<int32_t>(k ? 0 : rows);
+  w.zt = c.take<float>(k ? 0 : rows);
   w.q = c.take<float>((size_t)rows * k);
   w.cw = c.take<float>((size_t)rows * k);
   w.idx = c.take<int32_t>((size_t)rows * k);
@@ -713,8 +980,9 @@ static FwdWs fwd_ws(void* ws, int rows, int vocab, int width, int k) {
 }
 
 // Classes per piece of the backward pass: the piece's dz takes 2 bytes per row and class; at most PIECE_BYTES, but not so few classes that
-// the products become short (4096).  Pieces are of nearly equal size.
-constexpr long long PIECE_BYTES = 512ll << 20;
+// the products become short (4096).  Pieces are of nearly equal size.  Fewer pieces are faster, as each one adds to the sums of dh in memory
+// and starts four kernels (16384 rows x 50257 x 2048: 10.2 ms in 2 pieces, 10.7 in 4, 12.8 in 13).
+constexpr long long PIECE_BYTES = 1ll << 30;
 static int piece_classes(int rows, int vocab) {
   long long most = PIECE_BYTES / (2 * pad_rows(rows));
   most = most < 4096 ? 4096 : most;
@@ -730,6 +998,7 @@ struct BwdWs {
   float* lse2;
   uint16_t* dz;
   float* acc;
+  float* slots;
   int piece;
   size_t bytes;
 };
@@ -742,6 +1011,8 @@ static BwdWs bwd_ws(void* ws, int rows, int vocab, int width) {
   w.lse2 = c.take<float>(pad_rows(rows));
   w.dz = c.take<uint16_t>((size_t)pad_rows(rows) * w.piece);
   w.acc = c.take<float>(w.piece < vocab ? (size_t)pad_rows(rows) * width : 0);
+  const bool split = (w.piece < vocab ? w.piece : vocab) > SPLIT_MIN_KB * BK || rows > SPLIT_MIN_KB * BK;
+  w.slots = c.take<float>(split ? (size_t)2 * sm_count() * BM * BN : 0);   // two tiles' parts per worker
   w.bytes = c.used + 256;
   return w;
 }
@@ -791,15 +1062,15 @@ static int finish_launch(const FwdArgs& a, const FwdWs& w, int n_part, cudaStrea
   const T* packed = reinterpret_cast<const T*>(w.packed);
   const T* weight = static_cast<const T*>(a.weight);
   auto go = [&](auto kernel, int rows_per_block) {
-    launch_chained(kernel, dim3((a.rows + rows_per_block - 1) / rows_per_block), dim3(kFinishThreads), 0, st,
+    const size_t smem = a.target ? 0 : (size_t)rows_per_block * a.k * sizeof(float);   // at most 16 KB
+    launch_chained(kernel, dim3((a.rows + rows_per_block - 1) / rows_per_block), dim3(kFinishThreads), smem, st,
                    static_cast<const float2*>(w.part), pad_rows(a.rows), n_part, static_cast<const int32_t*>(a.pos + a.rows),
-                   static_cast<const int32_t*>(w.origin), packed, pad_width(a.width), weight, a.ldw, a.width, a.target,
-                   static_cast<const int32_t*>(w.idx), static_cast<const float*>(w.q), static_cast<const float*>(w.cw), a.k, a.inv_t,
+                   static_cast<const int32_t*>(w.origin), packed, pad_width(a.width), weight, a.ldw, a.width,
+                   static_cast<const int32_t*>(w.tgt), static_cast<const float*>(w.zt), static_cast<const int32_t*>(a.target ? nullptr : w.idx), static_cast<const float*>(w.q), static_cast<const float*>(w.cw), a.k, a.inv_t,
                    a.loss_rows, a.lse_rows, a.diff);
     return launch_status("finish_rows_kernel");
   };
-  // 32 rows a block read the partial sums in whole lines; with few rows, more blocks
-  if (a.rows >= 2048) return go(finish_rows_kernel<T, 32>, 32);
+  // 8 rows a block read the partial sums in whole sectors; with few rows, more blocks
   if (a.rows >= 256) return go(finish_rows_kernel<T, 8>, 8);
   return go(finish_rows_kernel<T, 1>, 1);
 }
@@ -818,7 +1089,7 @@ static int linear_fwd(const char* fn, const FwdArgs& a, cudaStream_t st) {
   blocks = blocks > 4 * 148 ? 4 * 148 : blocks;
   launch_chained(pack_rows_kernel, dim3(blocks), dim3(kRowThreads), 0, st, static_cast<const uint16_t*>(a.hidden), a.ldh, a.target,
                  static_cast<const int32_t*>(a.target ? nullptr : w.live), a.rows, a.vocab, a.width, w.packed, pad_width(a.width), w.origin,
-                 a.pos, a.loss_rows, a.lse_rows);
+                 w.tgt, a.pos, a.loss_rows, a.lse_rows);
   if (int rc = launch_status("pack_rows_kernel")) return rc;
   const bool paired = paired_for(a.rows);
   CUtensorMap tmA, tmB;
@@ -832,8 +1103,10 @@ static int linear_fwd(const char* fn, const FwdArgs& a, cudaStream_t st) {
   p.c = a.inv_t * kLog2e;
   p.part = w.part;
   p.part_ld = pad_rows(a.rows);
-  int rc = a.dtype == LANCET_BF16 ? launch_product<__nv_bfloat16, FORM_Z, EPI_LSE>(tmA, tmB, p, a.rows, a.vocab, paired, st)
-                                  : launch_product<__half, FORM_Z, EPI_LSE>(tmA, tmB, p, a.rows, a.vocab, paired, st);
+  p.tgt = a.target ? w.tgt : nullptr;
+  p.zt = w.zt;
+  int rc = a.dtype == LANCET_BF16 ? launch_product<__nv_bfloat16, FORM_Z, EPI_LSE>(tmA, tmB, p, a.rows, a.vocab, a.width, paired, st)
+                                  : launch_product<__half, FORM_Z, EPI_LSE>(tmA, tmB, p, a.rows, a.vocab, a.width, paired, st);
   if (rc) return rc;
   const int n_part = 2 * ((a.vocab + BN - 1) / BN);
   rc = a.dtype == LANCET_BF16 ? finish_launch<__nv_bfloat16>(a, w, n_part, st) : finish_launch<__half>(a, w, n_part, st);
@@ -867,7 +1140,7 @@ struct BwdArgs {
 template <typename T>
 static int linear_bwd_t(const BwdArgs& a, const BwdWs& w, cudaStream_t st) {
   int blocks = (a.rows + 7) / 8;
-  blocks = blocks > 4 * 148 ? 4 * 148 : blocks;
+  blocks = blocks > 4 * 148 ? 4 * 148 : (blocks < 8 ? 8 : blocks);   // the zero rows want some warps even for one row
   launch_chained(repack_rows_kernel, dim3(blocks), dim3(kRowThreads), 0, st, static_cast<const uint16_t*>(a.hidden), a.ldh, a.pos, a.lse_rows,
                  a.rows, a.width, w.packed, pad_width(a.width), w.origin, w.lse2, static_cast<uint16_t*>(a.dhidden));
   if (int rc = launch_status("repack_rows_kernel")) return rc;
@@ -888,6 +1161,7 @@ static int linear_bwd_t(const BwdArgs& a, const BwdWs& w, cudaStream_t st) {
   p.dz_ld = w.piece;
   p.grad_out = a.grad_out;
   p.inv_live = a.inv_live;
+  p.slots = w.slots;
   p.scale = a.scale / (a.inv_t * unit);
   CUtensorMap hK, wK, dzK, wMN, dzMN, hMN;
   if (int rc = make_map(&hK, w.packed, padded, a.width, pad_width(a.width), BM, a.dtype)) return rc;
@@ -901,7 +1175,7 @@ static int linear_bwd_t(const BwdArgs& a, const BwdWs& w, cudaStream_t st) {
     const bool last = v0 + classes == a.vocab;
     p.class0 = v0;
     p.classes = classes;
-    if (int rc = launch_product<T, FORM_Z, EPI_PROB>(hK, wK, p, a.rows, classes, paired, st)) return rc;
+    if (int rc = launch_product<T, FORM_Z, EPI_PROB>(hK, wK, p, a.rows, classes, a.width, paired, st)) return rc;
     const long long entries = (long long)a.rows * a.k;
     launch_chained(place_targets_kernel<T>, dim3((unsigned)((entries + 255) / 256)), dim3(256), 0, st, static_cast<const int32_t*>(p.count),
                    static_cast<const int32_t*>(w.origin), a.target, a.loss_rows, a.indices, a.diff, a.k, v0, classes, unit,
@@ -916,11 +1190,11 @@ static int linear_bwd_t(const BwdArgs& a, const BwdWs& w, cudaStream_t st) {
       ph.acc_out = !last;
     }
     if (a.dhidden)
-      if (int rc = launch_product<T, FORM_DH, EPI_OUT>(dzK, wMN, ph, a.rows, a.width, paired, st)) return rc;
+      if (int rc = launch_product<T, FORM_DH, EPI_OUT>(dzK, wMN, ph, a.rows, a.width, classes, paired, st)) return rc;
     if (!a.dweight) continue;
     Params pw = p;
     pw.out = a.dweight;
-    if (int rc = launch_product<T, FORM_DW, EPI_OUT>(dzMN, hMN, pw, classes, a.width, paired_for(classes), st)) return rc;
+    if (int rc = launch_product<T, FORM_DW, EPI_OUT>(dzMN, hMN, pw, classes, a.width, a.rows, paired_for(classes), st)) return rc;
   }
   return LANCET_OK;
 }

@@ -10,7 +10,6 @@ torch supplies device memory and the current stream only; all arithmetic runs in
 library behind the C ABI.  Extra keyword arguments (k, gates dtype) extend the surface to the
 top-2 gate; their defaults reproduce the reference ops.
 """
-import contextlib
 import ctypes
 
 import torch
@@ -345,64 +344,61 @@ def softmax_xent_bwd(logits, target, vocab, lse, grad_out, scale):
     return dx
 
 
-def _on(t):
-    """The tensor's device as the current one, where it is not."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
-def _matrix(name, what, t, like=None):
+def _matrix(name, what, t):
     """A [rows, cols] CUDA matrix with adjacent columns (copied where they are not) and its row stride."""
     if not t.is_cuda:
         raise ValueError("lancet_b200 ops need CUDA tensors (there is no CPU path)")
     if t.dim() != 2:
         raise ValueError("%s: %s must be a matrix" % (name, what))
-    if like is not None and t.device != like.device:
-        raise ValueError("%s: %s is on %s, the first operand on %s" % (name, what, t.device, like.device))
-    rows, cols = t.shape
-    if rows > 1 and t.stride(0) < cols or cols > 1 and t.stride(1) != 1:
+    if t.is_contiguous():
+        return t, t.shape[1]
+    if t.stride(1) != 1 or t.stride(0) < t.shape[1]:
         t = t.contiguous()
-    return t, max(t.stride(0), cols)
+    return t, max(t.stride(0), t.shape[1])
 
 
 def _classes(name, vocab, most):
-    vocab = most if vocab is None else int(vocab)
+    if vocab is None:
+        return most
+    vocab = int(vocab)
     if not 1 <= vocab <= most:
         raise ValueError("%s: vocab=%d for %d classes" % (name, vocab, most))
     return vocab
 
 
 def _target_rows(name, target, like):
-    if not target.is_cuda or target.device != like.device or target.dtype != torch.int64 or target.shape != (like.shape[0],):
+    if target.dtype != torch.int64 or target.shape != (like.shape[0],) or target.device != like.device:
         raise TypeError("%s: target must be an int64 vector with an entry per row, on the operands' device" % name)
     return target.contiguous()
 
 
 def _teacher_rows(name, top_values, top_indices, like):
-    for t in (top_values, top_indices):
-        if not t.is_cuda or t.device != like.device or t.dim() != 2 or t.shape[0] != like.shape[0] or t.shape != top_indices.shape:
-            raise ValueError("%s: the teacher's values and indices must be [rows, k] on the operands' device" % name)
-    if top_indices.dtype != torch.int64:
-        raise TypeError("%s: top_indices must be int64" % name)
-    _dt(top_values)
+    if top_indices.dim() != 2 or top_values.shape != top_indices.shape or top_indices.shape[0] != like.shape[0] or \
+            top_values.device != like.device or top_indices.device != like.device:
+        raise ValueError("%s: the teacher's values and indices must be [rows, k] on the operands' device" % name)
+    if top_indices.dtype != torch.int64 or top_values.dtype not in _DT:
+        raise TypeError("%s: top_indices must be int64, the values float32, float16 or bfloat16" % name)
     return top_values.contiguous(), top_indices.contiguous()
 
 
-def _head_operands(name, hidden, weight):
-    """hidden [rows, width] and weight [classes, width] as the head's products read them: (hidden, its row stride, weight, its row
-    stride).  A weight whose rows do not start on 16-byte boundaries is copied to a padded row stride."""
+def _head_operands(name, hidden, weight, vocab):
+    """hidden [rows, width] and weight [classes, width] as the head's products read them, with their row strides, and the number of
+    classes.  A weight whose rows do not start on 16-byte boundaries is copied to a padded row stride."""
     hidden, ldh = _matrix(name, "hidden", hidden)
-    weight, ldw = _matrix(name, "weight", weight, hidden)
-    if hidden.dtype != weight.dtype or hidden.dtype not in (torch.bfloat16, torch.float16):
+    weight, ldw = _matrix(name, "weight", weight)
+    if hidden.dtype != weight.dtype or (hidden.dtype != torch.bfloat16 and hidden.dtype != torch.float16):
         raise TypeError("%s: bfloat16 or float16 operands of one type" % name)
-    if weight.shape[1] != hidden.shape[1] or hidden.shape[1] < 1 or weight.shape[0] < 1:
-        raise ValueError("%s: hidden [rows, width] and weight [classes, width] do not match: %s, %s"
+    classes, width = weight.shape
+    if width != hidden.shape[1] or width < 1 or classes < 1 or weight.device != hidden.device:
+        raise ValueError("%s: hidden [rows, width] and weight [classes, width] on one device do not match: %s, %s"
                          % (name, tuple(hidden.shape), tuple(weight.shape)))
+    vocab = _classes(name, vocab, classes)
     if ldw % 8 or weight.data_ptr() % 16:
-        ldw = (weight.shape[1] + 7) // 8 * 8
-        padded = torch.empty((weight.shape[0], ldw), dtype=weight.dtype, device=weight.device)
-        padded[:, :weight.shape[1]] = weight
+        ldw = (width + 7) // 8 * 8
+        padded = torch.empty((classes, ldw), dtype=weight.dtype, device=weight.device)
+        padded[:, :width] = weight
         weight = padded
-    return hidden, ldh, weight, ldw
+    return hidden, ldh, weight, ldw, vocab
 
 
 def _head_status(device):
@@ -414,13 +410,82 @@ def _head_status(device):
 
 
 def _grad_scalar(name, t, like):
-    if t is not None and (t.dtype != torch.float32 or t.numel() != 1 or t.device != like.device):
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.numel() != 1 or t.device != like.device:
         raise TypeError("%s: grad_out and inv_live must be float32 scalars on the operands' device" % name)
-    return _ptr(t)
+    return t.data_ptr()
 
 
-def _row_floats(like, *shape):
-    return torch.empty(shape, dtype=torch.float32, device=like.device)
+def _launch(fn, like, *args):
+    """fn(*args, stream) on the tensor's device and its current stream."""
+    index = like.device.index
+    if index == torch.cuda.current_device():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        with torch.cuda.device(index):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+
+
+def _state(like, rows, k):
+    """What a forward pass leaves behind, in one float32 allocation: loss_rows, lse_rows, inv_live, pos (int32, rows + 1), and k numbers per
+    row; with the mean as a tensor of its own."""
+    device = like.device
+    return (torch.empty((), dtype=torch.float32, device=device), torch.empty(rows * (3 + k) + 2, dtype=torch.float32, device=device))
+
+
+def _state_parts(state, rows, k):
+    """(loss_rows, lse_rows, inv_live, pos, the k numbers per row) as views."""
+    loss, lse, inv_live, pos, more = state.split((rows, rows, 1, rows + 1, rows * k))
+    return loss, lse, inv_live, pos.view(torch.int32), more.view(rows, k)
+
+
+def _state_ptrs(state, rows):
+    p = state.data_ptr()
+    return p, p + 4 * rows, p + 8 * rows, p + 8 * rows + 4, p + 12 * rows + 8
+
+
+def _linear_fwd(name, hidden, weight, vocab, target=None, teacher=None, temperature=1.0):
+    """Forward pass of the linear losses: (mean, state, operands as the kernels read them)."""
+    hidden, ldh, w, ldw, vocab = _head_operands(name, hidden, weight, vocab)
+    rows, width = hidden.shape
+    L = _capi.lib()
+    if teacher is None:
+        target, k = _target_rows(name, target, hidden), 0
+    else:
+        values, target = _teacher_rows(name, *teacher, hidden)
+        k = target.shape[1]
+    mean, state = _state(hidden, rows, k)
+    loss, lse, inv_live, pos, diff = _state_ptrs(state, rows)
+    nws = L.lancet_linear_loss_fwd_workspace_bytes(rows, vocab, width, k)
+    ws = torch.empty(nws, dtype=torch.uint8, device=hidden.device)
+    operands = (hidden.data_ptr(), ldh, w.data_ptr(), ldw)
+    end = (mean.data_ptr(), inv_live, ws.data_ptr(), nws, _head_status(hidden.device).data_ptr())
+    if teacher is None:
+        _launch(L.lancet_linear_xent_fwd, hidden, *operands, target.data_ptr(), rows, vocab, width, _DT[hidden.dtype], loss, lse, pos, *end)
+    else:
+        _launch(L.lancet_linear_distill_fwd, hidden, *operands, values.data_ptr(), _DT[values.dtype], target.data_ptr(), k, float(temperature),
+                rows, vocab, width, _DT[hidden.dtype], loss, lse, diff, pos, *end)
+    return mean, state, hidden, w, target, vocab
+
+
+def _linear_bwd(name, hidden, ldh, w, ldw, classes, vocab, target, loss, lse, pos, diff, k, temperature, grad_out, inv_live, scale,
+                need_hidden, need_weight):
+    """Backward pass on checked operands; loss, lse, pos, diff, grad_out and inv_live are device addresses."""
+    rows, width = hidden.shape
+    dh = torch.empty((rows, width), dtype=hidden.dtype, device=hidden.device) if need_hidden else None
+    dw = torch.empty((classes, width), dtype=hidden.dtype, device=hidden.device) if need_weight else None
+    L = _capi.lib()
+    nws = L.lancet_linear_loss_bwd_workspace_bytes(rows, vocab, width)
+    ws = torch.empty(nws, dtype=torch.uint8, device=hidden.device)
+    end = (rows, vocab, classes, width, _DT[hidden.dtype], grad_out, inv_live, scale, None if dh is None else dh.data_ptr(),
+           None if dw is None else dw.data_ptr(), ws.data_ptr(), nws, _head_status(hidden.device).data_ptr())
+    if diff is None:
+        _launch(L.lancet_linear_xent_bwd, hidden, hidden.data_ptr(), ldh, w.data_ptr(), ldw, target.data_ptr(), loss, lse, pos, *end)
+    else:
+        _launch(L.lancet_linear_distill_bwd, hidden, hidden.data_ptr(), ldh, w.data_ptr(), ldw, target.data_ptr(), diff, k, temperature, lse,
+                pos, *end)
+    return dh, dw
 
 
 def linear_xent_fwd(hidden, weight, target, vocab=None):
@@ -429,47 +494,9 @@ def linear_xent_fwd(hidden, weight, target, vocab=None):
     inv_live, pos): row losses and log-sum-exp (0 in ignored rows), the mean over the other rows, 1 / their number, and the int32 row list
     that `linear_xent_bwd` takes.  The workspace is allocated per call: calls on other streams and captured graphs share nothing.  As with
     the grouped GEMM a wait that ran out is recorded in `gemm_status`."""
-    name = "linear_xent_fwd"
-    hidden, ldh, w, ldw = _head_operands(name, hidden, weight)
-    vocab = _classes(name, vocab, weight.shape[0])
-    target = _target_rows(name, target, hidden)
-    rows, width = hidden.shape
-    loss, lse, mean, inv_live = (_row_floats(hidden, *s) for s in ((rows,), (rows,), (), ()))
-    pos = torch.empty((rows + 1,), dtype=torch.int32, device=hidden.device)
-    L = _capi.lib()
-    with _on(hidden):
-        nws = L.lancet_linear_loss_fwd_workspace_bytes(rows, vocab, width, 0)
-        ws = torch.empty(nws, dtype=torch.uint8, device=hidden.device)
-        check(L.lancet_linear_xent_fwd(_ptr(hidden), ldh, _ptr(w), ldw, _ptr(target), rows, vocab, width, _dt(hidden), _ptr(loss), _ptr(lse),
-                                       _ptr(pos), _ptr(mean), _ptr(inv_live), _ptr(ws), nws, _ptr(_head_status(hidden.device)),
-                                       _stream(hidden)))
+    mean, state, hidden = _linear_fwd("linear_xent_fwd", hidden, weight, vocab, target=target)[:3]
+    loss, lse, inv_live, pos, _ = _state_parts(state, hidden.shape[0], 0)
     return loss, lse, mean, inv_live, pos
-
-
-def linear_xent_bwd(hidden, weight, target, loss_rows, lse_rows, pos, vocab=None, grad_out=None, inv_live=None, scale=1.0,
-                    need_hidden=True, need_weight=True):
-    """Gradients (dhidden, dweight) of sum(loss_rows) * grad_out * inv_live * scale for `linear_xent_fwd`, in the operands' type; what is
-    not needed is None.  grad_out and inv_live: float32 scalars on the device, or None for 1.  Weight rows from `vocab` on and
-    hidden rows of ignored rows get zeros."""
-    name = "linear_xent_bwd"
-    hidden, ldh, w, ldw = _head_operands(name, hidden, weight)
-    vocab = _classes(name, vocab, weight.shape[0])
-    target = _target_rows(name, target, hidden)
-    _require_cuda(loss_rows, lse_rows, pos)
-    rows, width = hidden.shape
-    if loss_rows.shape != (rows,) or lse_rows.shape != (rows,) or pos.shape != (rows + 1,):
-        raise ValueError("%s: loss_rows, lse_rows and pos must be those of the forward call" % name)
-    dh = torch.empty((rows, width), dtype=hidden.dtype, device=hidden.device) if need_hidden else None
-    dw = torch.empty(tuple(weight.shape), dtype=weight.dtype, device=weight.device) if need_weight else None
-    L = _capi.lib()
-    with _on(hidden):
-        nws = L.lancet_linear_loss_bwd_workspace_bytes(rows, vocab, width)
-        ws = torch.empty(nws, dtype=torch.uint8, device=hidden.device)
-        check(L.lancet_linear_xent_bwd(_ptr(hidden), ldh, _ptr(w), ldw, _ptr(target), _ptr(loss_rows), _ptr(lse_rows), _ptr(pos), rows, vocab,
-                                       weight.shape[0], width, _dt(hidden), _grad_scalar(name, grad_out, hidden),
-                                       _grad_scalar(name, inv_live, hidden), float(scale), _ptr(dh), _ptr(dw), _ptr(ws), nws,
-                                       _ptr(_head_status(hidden.device)), _stream(hidden)))
-    return dh, dw
 
 
 def linear_distill_fwd(hidden, weight, top_values, top_indices, temperature=1.0, vocab=None):
@@ -478,63 +505,76 @@ def linear_distill_fwd(hidden, weight, top_values, top_indices, temperature=1.0,
     top_values [rows, k] float32, float16 or bfloat16, top_indices [rows, k] int64, k <= 512; an index that names no class does not
     count (NaN in its value included), a row without counting entries is ignored.  Returns (loss_rows, lse_rows, mean, inv_live, pos, diff)
     as `linear_xent_fwd` does; diff [rows, k] float32 is the student's minus the teacher's probability at the entries."""
-    name = "linear_distill_fwd"
-    hidden, ldh, w, ldw = _head_operands(name, hidden, weight)
-    vocab = _classes(name, vocab, weight.shape[0])
-    top_values, top_indices = _teacher_rows(name, top_values, top_indices, hidden)
-    (rows, width), k = hidden.shape, top_indices.shape[1]
-    loss, lse, mean, inv_live, diff = (_row_floats(hidden, *s) for s in ((rows,), (rows,), (), (), (rows, k)))
-    pos = torch.empty((rows + 1,), dtype=torch.int32, device=hidden.device)
-    L = _capi.lib()
-    with _on(hidden):
-        nws = L.lancet_linear_loss_fwd_workspace_bytes(rows, vocab, width, k)
-        ws = torch.empty(nws, dtype=torch.uint8, device=hidden.device)
-        check(L.lancet_linear_distill_fwd(_ptr(hidden), ldh, _ptr(w), ldw, _ptr(top_values), _dt(top_values), _ptr(top_indices), k,
-                                          float(temperature), rows, vocab, width, _dt(hidden), _ptr(loss), _ptr(lse), _ptr(diff), _ptr(pos),
-                                          _ptr(mean), _ptr(inv_live), _ptr(ws), nws, _ptr(_head_status(hidden.device)), _stream(hidden)))
+    mean, state, hidden, _, top_indices, _ = _linear_fwd("linear_distill_fwd", hidden, weight, vocab, teacher=(top_values, top_indices),
+                                                         temperature=temperature)
+    loss, lse, inv_live, pos, diff = _state_parts(state, hidden.shape[0], top_indices.shape[1])
     return loss, lse, mean, inv_live, pos, diff
+
+
+def _check_saved(name, hidden, lse_rows, pos, *more):
+    rows = hidden.shape[0]
+    _require_cuda(lse_rows, pos, *more)
+    if any(t.device != hidden.device for t in (lse_rows, pos, *more)) or any(t.dtype != torch.float32 for t in (lse_rows, *more)) or \
+            pos.dtype != torch.int32 or lse_rows.shape != (rows,) or pos.shape != (rows + 1,) or any(t.shape[0] != rows for t in more):
+        raise ValueError("%s: the saved tensors must be those of the forward call" % name)
+
+
+def linear_xent_bwd(hidden, weight, target, loss_rows, lse_rows, pos, vocab=None, grad_out=None, inv_live=None, scale=1.0,
+                    need_hidden=True, need_weight=True):
+    """Gradients (dhidden, dweight) of sum(loss_rows) * grad_out * inv_live * scale for `linear_xent_fwd`, in the operands' type; what is
+    not needed is None.  grad_out and inv_live: float32 scalars on the device, or None for 1.  Weight rows from `vocab` on and
+    hidden rows of ignored rows get zeros.  loss_rows, lse_rows and pos must be the forward call's on the same inputs."""
+    name = "linear_xent_bwd"
+    classes = weight.shape[0]
+    hidden, ldh, w, ldw, vocab = _head_operands(name, hidden, weight, vocab)
+    target = _target_rows(name, target, hidden)
+    _check_saved(name, hidden, lse_rows, pos, loss_rows)
+    return _linear_bwd(name, hidden, ldh, w, ldw, classes, vocab, target, loss_rows.data_ptr(), lse_rows.data_ptr(), pos.data_ptr(), None, 0,
+                       1.0, _grad_scalar(name, grad_out, hidden), _grad_scalar(name, inv_live, hidden), float(scale), need_hidden, need_weight)
 
 
 def linear_distill_bwd(hidden, weight, top_indices, diff, lse_rows, pos, temperature=1.0, vocab=None, grad_out=None, inv_live=None,
                        scale=1.0, need_hidden=True, need_weight=True):
     """Gradients (dhidden, dweight) of `linear_distill_fwd`, as `linear_xent_bwd` gives them."""
     name = "linear_distill_bwd"
-    hidden, ldh, w, ldw = _head_operands(name, hidden, weight)
-    vocab = _classes(name, vocab, weight.shape[0])
+    classes = weight.shape[0]
+    hidden, ldh, w, ldw, vocab = _head_operands(name, hidden, weight, vocab)
     _, top_indices = _teacher_rows(name, diff, top_indices, hidden)
-    _require_cuda(diff, lse_rows, pos)
-    (rows, width), k = hidden.shape, top_indices.shape[1]
-    if diff.dtype != torch.float32 or lse_rows.shape != (rows,) or pos.shape != (rows + 1,):
-        raise ValueError("%s: diff, lse_rows and pos must be those of the forward call" % name)
-    dh = torch.empty((rows, width), dtype=hidden.dtype, device=hidden.device) if need_hidden else None
-    dw = torch.empty(tuple(weight.shape), dtype=weight.dtype, device=weight.device) if need_weight else None
-    L = _capi.lib()
-    with _on(hidden):
-        nws = L.lancet_linear_loss_bwd_workspace_bytes(rows, vocab, width)
-        ws = torch.empty(nws, dtype=torch.uint8, device=hidden.device)
-        check(L.lancet_linear_distill_bwd(_ptr(hidden), ldh, _ptr(w), ldw, _ptr(top_indices), _ptr(diff), k, float(temperature), _ptr(lse_rows),
-                                          _ptr(pos), rows, vocab, weight.shape[0], width, _dt(hidden), _grad_scalar(name, grad_out, hidden),
-                                          _grad_scalar(name, inv_live, hidden), float(scale), _ptr(dh), _ptr(dw), _ptr(ws), nws,
-                                          _ptr(_head_status(hidden.device)), _stream(hidden)))
-    return dh, dw
+    _check_saved(name, hidden, lse_rows, pos, diff)
+    return _linear_bwd(name, hidden, ldh, w, ldw, classes, vocab, top_indices, None, lse_rows.data_ptr(), pos.data_ptr(), diff.data_ptr(),
+                       top_indices.shape[1], float(temperature), _grad_scalar(name, grad_out, hidden), _grad_scalar(name, inv_live, hidden),
+                       float(scale), need_hidden, need_weight)
+
+
+def _distill_fwd(logits, top_values, top_indices, temperature, vocab):
+    name = "distill_fwd"
+    logits, ld = _matrix(name, "logits", logits)
+    dt = _dt(logits)
+    vocab = _classes(name, vocab, logits.shape[1])
+    values, indices = _teacher_rows(name, top_values, top_indices, logits)
+    rows, k = logits.shape[0], indices.shape[1]
+    mean, state = _state(logits, rows, k)
+    loss, lse, inv_live, live, weights = _state_ptrs(state, rows)
+    _launch(_capi.lib().lancet_distill_fwd, logits, logits.data_ptr(), ld, values.data_ptr(), _DT[values.dtype], indices.data_ptr(), k,
+            float(temperature), rows, vocab, dt, loss, lse, weights, live, mean.data_ptr(), inv_live)
+    return mean, state, logits, indices, vocab
+
+
+def _distill_bwd(logits, ld, indices, vocab, weights, live, lse, temperature, grad_out, inv_live, scale):
+    rows, cols = logits.shape
+    dx = torch.empty((rows, cols), dtype=logits.dtype, device=logits.device)
+    _launch(_capi.lib().lancet_distill_bwd, logits, logits.data_ptr(), ld, indices.data_ptr(), weights, live, indices.shape[1], temperature,
+            rows, vocab, cols, _DT[logits.dtype], lse, grad_out, inv_live, scale, dx.data_ptr(), cols)
+    return dx
 
 
 def distill_fwd(logits, top_values, top_indices, temperature=1.0, vocab=None):
     """The loss of `linear_distill_fwd` on given logits [rows, cols] (float32, float16 or bfloat16; columns from `vocab` on are padding
     and never read).  Returns (loss_rows, lse_rows, mean, inv_live, live_rows, class_weights); the last two are kept for `distill_bwd`."""
-    name = "distill_fwd"
-    logits, ld = _matrix(name, "logits", logits)
-    dt = _dt(logits)
-    vocab = _classes(name, vocab, logits.shape[1])
-    top_values, top_indices = _teacher_rows(name, top_values, top_indices, logits)
-    rows, k = logits.shape[0], top_indices.shape[1]
-    loss, lse, mean, inv_live, weights = (_row_floats(logits, *s) for s in ((rows,), (rows,), (), (), (rows, k)))
-    live = torch.empty((rows,), dtype=torch.int32, device=logits.device)
-    with _on(logits):
-        check(_capi.lib().lancet_distill_fwd(_ptr(logits), ld, _ptr(top_values), _dt(top_values), _ptr(top_indices), k, float(temperature),
-                                             rows, vocab, dt, _ptr(loss), _ptr(lse), _ptr(weights), _ptr(live), _ptr(mean), _ptr(inv_live),
-                                             _stream(logits)))
-    return loss, lse, mean, inv_live, live, weights
+    mean, state, logits, indices, _ = _distill_fwd(logits, top_values, top_indices, temperature, vocab)
+    rows = logits.shape[0]
+    loss, lse, inv_live, live, weights = _state_parts(state, rows, indices.shape[1])
+    return loss, lse, mean, inv_live, live[:rows], weights
 
 
 def distill_bwd(logits, top_indices, class_weights, live_rows, lse_rows, temperature=1.0, vocab=None, grad_out=None, inv_live=None,
@@ -543,19 +583,15 @@ def distill_bwd(logits, top_indices, class_weights, live_rows, lse_rows, tempera
     ignored rows are zero."""
     name = "distill_bwd"
     logits, ld = _matrix(name, "logits", logits)
-    dt = _dt(logits)
+    _dt(logits)
     vocab = _classes(name, vocab, logits.shape[1])
-    _, top_indices = _teacher_rows(name, class_weights, top_indices, logits)
+    _, indices = _teacher_rows(name, class_weights, top_indices, logits)
     _require_cuda(class_weights, live_rows, lse_rows)
-    (rows, cols), k = logits.shape, top_indices.shape[1]
-    if class_weights.dtype != torch.float32 or lse_rows.shape != (rows,) or live_rows.shape != (rows,):
+    if class_weights.dtype != torch.float32 or lse_rows.dtype != torch.float32 or live_rows.dtype != torch.int32 or \
+            lse_rows.shape != logits.shape[:1] or live_rows.shape != logits.shape[:1]:
         raise ValueError("%s: class_weights, live_rows and lse_rows must be those of the forward call" % name)
-    dx = torch.empty((rows, cols), dtype=logits.dtype, device=logits.device)
-    with _on(logits):
-        check(_capi.lib().lancet_distill_bwd(_ptr(logits), ld, _ptr(top_indices), _ptr(class_weights), _ptr(live_rows), k, float(temperature),
-                                             rows, vocab, cols, dt, _ptr(lse_rows), _grad_scalar(name, grad_out, logits),
-                                             _grad_scalar(name, inv_live, logits), float(scale), _ptr(dx), cols, _stream(logits)))
-    return dx
+    return _distill_bwd(logits, ld, indices, vocab, class_weights.data_ptr(), live_rows.data_ptr(), lse_rows.data_ptr(), float(temperature),
+                        _grad_scalar(name, grad_out, logits), _grad_scalar(name, inv_live, logits), float(scale))
 
 
 ACT = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3}

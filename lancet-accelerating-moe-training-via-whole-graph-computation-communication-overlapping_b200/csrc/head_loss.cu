@@ -23,6 +23,7 @@ using namespace lancet::gemm;
 constexpr int BM = 128, BN = 256, BK = 64, UMMA_K = 16;
 constexpr int A_STAGE_BYTES = BM * BK * 2;
 constexpr int EPI_WARPS = 8;
+constexpr int STAGE_OUT_LD = 17;                // words of a staged output row: 32 16-bit elements and one word against bank conflicts
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int TMEM_COLS = 512;
 constexpr int ROW_PAD = 256;                    // row buffers hold a multiple of this: whole tiles, in the paired form too
@@ -42,7 +43,7 @@ struct Cfg {
   static constexpr int B_STAGE_BYTES = B_COLS * BK * 2;
   static constexpr int STAGE_BYTES = A_STAGE_BYTES + B_STAGE_BYTES;
   static constexpr int SMEM_DATA = STAGES * STAGE_BYTES;
-  static constexpr int SMEM_BYTES = SMEM_DATA + 1024 + 256;
+  static constexpr int SMEM_BYTES = SMEM_DATA + 1024 /*alignment slack*/ + 256 /*barriers*/ + EPI_WARPS * 32 * STAGE_OUT_LD * 4;
 };
 
 struct Params {
@@ -69,6 +70,7 @@ struct Params {
   const float* inv_live;
   float scale;
   float* acc;               // float32 sums over the pieces, or null
+  long long acc_ld;
   int acc_in, acc_out;      // add the sums so far / store sums instead of the output
   float* slots;             // partial sums of split tiles
 };
@@ -328,138 +330,65 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   } else {
     // ---------------- epilogue: TMEM lane quadrant = warp % 4, column half = (warp - 2) / 4; a thread owns one row ----------------
     const int quad = warp & 3, half = (warp - 2) >> 2;
-    constexpr int CHUNKS = BN / 64;   // 32-column chunks of a half tile
     int buf = 0;
     uint32_t tphase = 0;
     bool ok = true;
     float g = 1.f;
     if (EPI == EPI_OUT) g = p.scale * (p.grad_out ? *p.grad_out : 1.f) * (p.inv_live ? *p.inv_live : 1.f);
-    auto release = [&]() {   // the accumulator may be overwritten once every epilogue warp (of both CTAs) has read it
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (CTA2) mbar_arrive_cluster(cluster_addr(bar_tempty + 8 * buf, 0)); else mbar_arrive(bar_tempty + 8 * buf);
-      }
-      tphase ^= 1u << buf;
-      buf ^= 1;
-    };
+    // rows of the output on 32-byte boundaries: each thread stores its own; else they pass through shared memory
     const bool vec = p.width % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
+    const bool pairs = p.width % 2 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 3) == 0;
+    uint32_t* stage_out = reinterpret_cast<uint32_t*>(smem + C::SMEM_DATA + 256) + (warp - 2) * 32 * STAGE_OUT_LD;
     const uint32_t acc_mask = d.kb > 0 ? 0xffffffffu : 0u;   // no live rows: the accumulator holds stale values
     while (ok && walk.step()) {
       const Tile tl = decode<FORM, CTA2>(p, d, walk.t, rank);
       const int row = tl.mt * BM + quad * 32 + lane;
       const bool row_live = row < d.m;
       const int col_first = tl.nt * BN + half * (BN / 2);
+      const int left = d.n - col_first;   // columns of this half tile that exist
       float off = 0.f;
       long long out_row = row;
+      int want = -1;                      // EPI_LSE: column of the row's target in this half tile
       if (EPI == EPI_PROB && row_live) off = p.shift - p.lse2[row];
       if (EPI == EPI_OUT && row_live) out_row = p.row_map ? p.row_map[row] : (long long)p.class0 + row;
+      if (EPI == EPI_LSE && p.tgt && row_live) want = p.tgt[row] - col_first;
       ok = mbar_wait(bar_tfull + 8 * buf, (tphase >> buf) & 1, abort_flag, p.status, 14);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN + half * (BN / 2));
-      if (EPI == EPI_OUT && walk.slot >= 0) {
-        float* dst = p.slots + ((long long)walk.slot * (CTA2 ? 2 * BM : BM) + rank * BM + quad * 32 + lane) * BN + half * (BN / 2);
-#pragma unroll 1
-        for (int ch = 0; ch < CHUNKS; ++ch) {
-          uint32_t r[32];
-          tmem_ld32(taddr + ch * 32, r);
-          if (row_live) {
-#pragma unroll
-            for (int q = 0; q < 32; q += 8)
-              st_global_32B(dst + ch * 32 + q, make_uint4(r[q], r[q + 1], r[q + 2], r[q + 3]),
-                            make_uint4(r[q + 4], r[q + 5], r[q + 6], r[q + 7]));
-          }
+      auto release = [&]() {   // the accumulator may be overwritten once every epilogue warp (of both CTAs) has read it
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (CTA2) mbar_arrive_cluster(cluster_addr(bar_tempty + 8 * buf, 0)); else mbar_arrive(bar_tempty + 8 * buf);
         }
+        tphase ^= 1u << buf;
+        buf ^= 1;
+      };
+      // f(first column, 32 values) for the half tile's four chunks; the next chunk is on its way while one is worked on, and the accumulator
+      // goes back before the last one is
+      auto chunks = [&](auto&& f) {
+        uint32_t a[32], b[32];
+        tmem_ld32_async(taddr, a);
+        tmem_wait(a);
+        tmem_ld32_async(taddr + 32, b);
+        f(0, a);
+        __syncwarp();
+        tmem_wait(b);
+        tmem_ld32_async(taddr + 64, a);
+        f(32, b);
+        __syncwarp();
+        tmem_wait(a);
+        tmem_ld32_async(taddr + 96, b);
+        f(64, a);
+        __syncwarp();
+        tmem_wait(b);
         release();
-        continue;
-      }
-      if (EPI == EPI_OUT) {
-        // whole chunks of rows on 32-byte boundaries first: one loop without other control flow around the TMEM loads and the stores
-        const int left = d.n - col_first;
-        const int whole = ACC || !vec ? 0 : min(CHUNKS, left / 32);
-        T* dst = static_cast<T*>(p.out) + out_row * p.width + col_first;
-#pragma unroll 1
-        for (int ch = 0; ch < whole; ++ch) {
-          uint32_t r[32], o[16];
-          tmem_ld32(taddr + ch * 32, r);
-#pragma unroll
-          for (int i = 0; i < 32; i += 2)
-            o[i >> 1] = pack_pair<T>(__uint_as_float(r[i] & acc_mask) * g, __uint_as_float(r[i + 1] & acc_mask) * g);
-          if (row_live) {
-#pragma unroll
-            for (int q = 0; q < 4; q += 2)
-              st_global_32B(dst + ch * 32 + 8 * q, make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]),
-                            make_uint4(o[4 * q + 4], o[4 * q + 5], o[4 * q + 6], o[4 * q + 7]));
-          }
-        }
-#pragma unroll 1
-        for (int ch = whole; ch < CHUNKS && ch * 32 < left; ++ch) {
-          uint32_t r[32];
-          tmem_ld32(taddr + ch * 32, r);
-          if (!row_live) continue;
-          float* acc = ACC ? p.acc + (long long)row * p.width + col_first + ch * 32 : nullptr;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (ch * 32 + i >= left) continue;
-            float v = __uint_as_float(r[i] & acc_mask);
-            if (ACC && p.acc_in) v += acc[i];
-            if (ACC && p.acc_out)
-              acc[i] = v;
-            else
-              dst[ch * 32 + i] = Num<T>::from_f(v * g);
-          }
-        }
-        release();
-        continue;
-      }
-      int want = -1;               // EPI_LSE: column of the row's target in this half tile
-      if (EPI == EPI_LSE && p.tgt && row_live) want = p.tgt[row] - col_first;
-      float m = -1e30f, s = 0.f;   // EPI_LSE: maximum of z and sum of 2^((z - m) c)
-#pragma unroll 1
-      for (int ch = 0; ch < CHUNKS; ++ch) {
-        uint32_t r[32];
-        tmem_ld32(taddr + ch * 32, r);
-        const int left = d.n - (col_first + ch * 32);   // columns of the chunk that exist
-        if (EPI == EPI_LSE) {
-          if (left < 32) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = i < left ? r[i] : 0xff800000u;
-          }
-          float mx = __uint_as_float(r[0]);
-#pragma unroll
-          for (int i = 1; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
-          mx = fmaxf(mx, m);
-          s *= ex2f((m - mx) * p.c);
-          m = mx;
-          const float mc = -m * p.c;
-          float s4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int i = 0; i < 32; ++i) s4[i & 3] += ex2f(fmaf(__uint_as_float(r[i]), p.c, mc));
-          s += (s4[0] + s4[1]) + (s4[2] + s4[3]);
-        } else if (EPI == EPI_PROB) {
-          uint32_t o[16];
-          const uint32_t keep = row_live ? 0xffffffffu : 0u;
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float a = ex2f(fmaf(__uint_as_float(r[i]), p.c, off)), b = ex2f(fmaf(__uint_as_float(r[i + 1]), p.c, off));
-            if (left < 32) {
-              a = i < left ? a : 0.f;
-              b = i + 1 < left ? b : 0.f;
-            }
-            o[i >> 1] = pack_pair<T>(a, b) & keep;
-          }
-          // the piece's buffer has whole tiles: every row and column of this one is written, zeros behind the last live ones
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.dz) + row * p.dz_ld + col_first + ch * 32);
-#pragma unroll
-          for (int q = 0; q < 4; q += 2)
-            st_global_32B(dst + q, make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]),
-                          make_uint4(o[4 * q + 4], o[4 * q + 5], o[4 * q + 6], o[4 * q + 7]));
-        }
-      }
+        f(96, b);
+      };
       if (EPI == EPI_LSE) {
-        // the few targets in this half tile: their columns once more
+        // the few targets in this half tile
         unsigned hits = __ballot_sync(0xffffffffu, want >= 0 && want < BN / 2);
         while (hits) {
           const int owner = __ffs(hits) - 1, col = __shfl_sync(0xffffffffu, want, owner);
@@ -467,9 +396,135 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           if (lane == owner) p.zt[row] = __uint_as_float(z);
           hits &= hits - 1;
         }
+        float m = -1e30f, s = 0.f;   // maximum of z and sum of 2^((z - m) c)
+        chunks([&](int c0, uint32_t(&r)[32]) {
+          if (left < c0 + 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = c0 + i < left ? r[i] : 0xff800000u;
+          }
+          float mx[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i] = fmaxf(__uint_as_float(r[i]), __uint_as_float(r[i + 4]));
+#pragma unroll
+          for (int i = 8; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(r[i]));
+          const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), m);
+          s *= ex2f((m - top) * p.c);
+          m = top;
+          const f32x2 cc = splat2(p.c), mc = splat2(-m * p.c);
+          f32x2 sum[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float x, y;
+            unpack2(fma2(pack2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), cc, mc), x, y);
+            sum[(i >> 1) & 3] = add2(sum[(i >> 1) & 3], pack2(ex2f(x), ex2f(y)));
+          }
+          float x, y;
+          unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), x, y);
+          s += x + y;
+        });
+        if (row_live) p.part[(long long)(2 * tl.nt + half) * p.part_ld + row] = make_float2(m * p.c, s);
+      } else if (EPI == EPI_PROB) {
+        // the piece's buffer has whole tiles: every row and column of this one is written, zeros behind the last live ones
+        T* dst = static_cast<T*>(p.dz) + row * p.dz_ld + col_first;
+        const uint32_t keep = row_live ? 0xffffffffu : 0u;
+        chunks([&](int c0, uint32_t(&r)[32]) {
+          uint32_t o[16];
+          const f32x2 cc = splat2(p.c), oo = splat2(off);
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float x, y;
+            unpack2(fma2(pack2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), cc, oo), x, y);
+            o[i >> 1] = pack_pair<T>(ex2f(x), ex2f(y)) & keep;
+          }
+          if (left < c0 + 32) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int have = left - c0 - 2 * i;
+              o[i] &= have >= 2 ? 0xffffffffu : (have == 1 ? 0x0000ffffu : 0u);
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < 16; q += 8)
+            st_global_32B(dst + c0 + 2 * q, make_uint4(o[q], o[q + 1], o[q + 2], o[q + 3]),
+                          make_uint4(o[q + 4], o[q + 5], o[q + 6], o[q + 7]));
+        });
+      } else if (walk.slot >= 0 || (ACC && p.acc_out)) {
+        // float32 results: a part of a split tile, or the sums over the pieces so far (row strides of whole tiles: no bounds)
+        const bool part = walk.slot >= 0;
+        float* dst = part ? p.slots + ((long long)walk.slot * (CTA2 ? 2 * BM : BM) + rank * BM + quad * 32 + lane) * BN + half * (BN / 2)
+                          : p.acc + row * p.acc_ld + col_first;
+        const bool add = ACC && !part && p.acc_in;
+        chunks([&](int c0, uint32_t(&r)[32]) {
+          if (!row_live) return;
+          if (add) {
+#pragma unroll
+            for (int q = 0; q < 32; q += 4) {
+              const float4 x = *reinterpret_cast<const float4*>(dst + c0 + q);
+              r[q] = __float_as_uint(__uint_as_float(r[q]) + x.x);
+              r[q + 1] = __float_as_uint(__uint_as_float(r[q + 1]) + x.y);
+              r[q + 2] = __float_as_uint(__uint_as_float(r[q + 2]) + x.z);
+              r[q + 3] = __float_as_uint(__uint_as_float(r[q + 3]) + x.w);
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < 32; q += 8)
+            st_global_32B(dst + c0 + q, make_uint4(r[q], r[q + 1], r[q + 2], r[q + 3]),
+                          make_uint4(r[q + 4], r[q + 5], r[q + 6], r[q + 7]));
+        });
+      } else {
+        T* dst = static_cast<T*>(p.out) + out_row * p.width + col_first;
+        chunks([&](int c0, uint32_t(&r)[32]) {
+          if (left <= c0) return;   // the same for the whole warp
+          uint32_t o[16];
+          if (ACC) {
+            const float* acc = p.acc + row * p.acc_ld + col_first + c0;
+            if (row_live) {
+#pragma unroll
+              for (int q = 0; q < 32; q += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(acc + q);
+                r[q] = __float_as_uint(__uint_as_float(r[q]) + x.x);
+                r[q + 1] = __float_as_uint(__uint_as_float(r[q + 1]) + x.y);
+                r[q + 2] = __float_as_uint(__uint_as_float(r[q + 2]) + x.z);
+                r[q + 3] = __float_as_uint(__uint_as_float(r[q + 3]) + x.w);
+              }
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            o[i >> 1] = pack_pair<T>(__uint_as_float(r[i] & acc_mask) * g, __uint_as_float(r[i + 1] & acc_mask) * g);
+          if (vec && left >= c0 + 32) {
+            if (row_live) {
+#pragma unroll
+              for (int q = 0; q < 16; q += 8)
+                st_global_32B(dst + c0 + 2 * q, make_uint4(o[q], o[q + 1], o[q + 2], o[q + 3]),
+                              make_uint4(o[q + 4], o[q + 5], o[q + 6], o[q + 7]));
+            }
+            return;
+          }
+          // the warp's 32 x 32 block through shared memory, stored row by row in neighbouring lanes
+#pragma unroll
+          for (int i = 0; i < 16; ++i) stage_out[lane * STAGE_OUT_LD + i] = o[i];
+          __syncwarp();
+          const int cols = min(32, left - c0), rows = min(32, d.m - (tl.mt * BM + quad * 32));
+          const unsigned long long at = reinterpret_cast<unsigned long long>(dst + c0);
+          if (pairs) {
+            const int sub = lane >> 4, w = lane & 15;
+#pragma unroll 4
+            for (int i = 0; i < 32; i += 2) {
+              uint32_t* to = reinterpret_cast<uint32_t*>(__shfl_sync(0xffffffffu, at, i + sub));
+              if (i + sub < rows && 2 * w < cols) to[w] = stage_out[(i + sub) * STAGE_OUT_LD + w];   // an even width has even `cols`
+            }
+          } else {
+            const uint16_t* st = reinterpret_cast<const uint16_t*>(stage_out);
+#pragma unroll 4
+            for (int i = 0; i < 32; ++i) {
+              uint16_t* to = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, at, i));
+              if (i < rows && lane < cols) to[lane] = st[2 * i * STAGE_OUT_LD + lane];
+            }
+          }
+          __syncwarp();
+        });
       }
-      if (EPI == EPI_LSE && row_live) p.part[(long long)(2 * tl.nt + half) * p.part_ld + row] = make_float2(m * p.c, s);
-      release();
     }
   }
   // ---------------- teardown ----------------
@@ -537,7 +592,7 @@ __global__ void __launch_bounds__(256) join_tiles_kernel(Params p, int workers) 
   auto finish = [&](int i, const float4& x) {
     const int row = mu * UNIT + i;
     const float v[4] = {x.x, x.y, x.z, x.w};
-    float* acc = p.acc + (long long)row * p.width + n0;
+    float* acc = p.acc + row * p.acc_ld + n0;
     T* out = static_cast<T*>(p.out) + (p.row_map ? p.row_map[row] : (long long)p.class0 + row) * p.width + n0;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -949,6 +1004,7 @@ struct Carver {
 };
 
 static long long pad_rows(long long rows) { return rows < 1 ? ROW_PAD : (rows + ROW_PAD - 1) / ROW_PAD * ROW_PAD; }
+static long long pad_cols(int width) { return (width + BN - 1) / BN * BN; }
 static int pad_width(int width) { return (width + 7) / 8 * 8; }
 
 struct FwdWs {
@@ -1010,7 +1066,7 @@ static BwdWs bwd_ws(void* ws, int rows, int vocab, int width) {
   w.origin = c.take<int32_t>(rows);
   w.lse2 = c.take<float>(pad_rows(rows));
   w.dz = c.take<uint16_t>((size_t)pad_rows(rows) * w.piece);
-  w.acc = c.take<float>(w.piece < vocab ? (size_t)pad_rows(rows) * width : 0);
+  w.acc = c.take<float>(w.piece < vocab ? (size_t)pad_rows(rows) * pad_cols(width) : 0);
   const bool split = (w.piece < vocab ? w.piece : vocab) > SPLIT_MIN_KB * BK || rows > SPLIT_MIN_KB * BK;
   w.slots = c.take<float>(split ? (size_t)2 * sm_count() * BM * BN : 0);   // two tiles' parts per worker
   w.bytes = c.used + 256;
@@ -1186,6 +1242,7 @@ static int linear_bwd_t(const BwdArgs& a, const BwdWs& w, cudaStream_t st) {
     ph.row_map = w.origin;
     if (w.piece < a.vocab) {
       ph.acc = w.acc;
+      ph.acc_ld = pad_cols(a.width);
       ph.acc_in = v0 > 0;
       ph.acc_out = !last;
     }

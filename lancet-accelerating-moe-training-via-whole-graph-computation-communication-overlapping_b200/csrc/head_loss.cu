@@ -23,7 +23,8 @@ using namespace lancet::gemm;
 constexpr int BM = 128, BN = 256, BK = 64, UMMA_K = 16;
 constexpr int A_STAGE_BYTES = BM * BK * 2;
 constexpr int EPI_WARPS = 8;
-constexpr int STAGE_OUT_LD = 17;                // words of a staged output row: 32 16-bit elements and one word against bank conflicts
+constexpr int OUT_BOX_ROWS = 32, OUT_BOX_BYTES = OUT_BOX_ROWS * 128;   // an epilogue warp's box on its way out: 32 rows x 64 16-bit elements
+constexpr int STAGE_OUT_LD = 17;                // words of a staged row where rows go out singly: 32 elements and one word against bank conflicts
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int TMEM_COLS = 512;
 constexpr int ROW_PAD = 256;                    // row buffers hold a multiple of this: whole tiles, in the paired form too
@@ -43,7 +44,7 @@ struct Cfg {
   static constexpr int B_STAGE_BYTES = B_COLS * BK * 2;
   static constexpr int STAGE_BYTES = A_STAGE_BYTES + B_STAGE_BYTES;
   static constexpr int SMEM_DATA = STAGES * STAGE_BYTES;
-  static constexpr int SMEM_BYTES = SMEM_DATA + 1024 /*alignment slack*/ + 256 /*barriers*/ + EPI_WARPS * 32 * STAGE_OUT_LD * 4;
+  static constexpr int SMEM_BYTES = SMEM_DATA + EPI_WARPS * OUT_BOX_BYTES + 1024 /*alignment slack*/ + 256 /*barriers*/;
 };
 
 struct Params {
@@ -58,13 +59,13 @@ struct Params {
   long long part_ld;
   const int32_t* tgt;     // target of every packed row, or null; its logit goes to zt
   float* zt;
-  // EPI_PROB: 2^(z c - lse2[row] + shift) of the piece
+  // EPI_PROB: 2^(z c - lse2[row] + shift) of the piece to tmOut, at the rows' targets (tgt) tdiff[row] instead
   const float* lse2;
+  const float* tdiff;
   float shift;
-  void* dz;
-  long long dz_ld;
   // EPI_OUT
   void* out;
+  int boxes;                // whole rows of the output go out through tmOut (rows on 16-byte boundaries, no row_map)
   const int32_t* row_map;   // output row of packed row i, or null
   const float* grad_out;
   const float* inv_live;
@@ -205,7 +206,8 @@ __device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) {
 // ACC (EPI_OUT): sums over the pieces pass through p.acc
 template <typename T, int FORM, int EPI, bool CTA2, bool ACC>
 __global__ void __launch_bounds__(THREADS, 1)
-head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, Params p) {
+head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmOut,
+                    Params p) {
   using C = Cfg<CTA2>;
   constexpr int STAGES = C::STAGES;
   constexpr bool A_MN = FORM == FORM_DW, B_MN = FORM != FORM_Z;
@@ -213,7 +215,8 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* sA = smem;
   unsigned char* sB = smem + STAGES * A_STAGE_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::SMEM_DATA);
+  unsigned char* sOut = smem + C::SMEM_DATA;   // a box per epilogue warp
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sOut + EPI_WARPS * OUT_BOX_BYTES);
   const uint32_t bar_full = smem_u32(bars), bar_empty = smem_u32(bars + STAGES);
   const uint32_t bar_tfull = smem_u32(bars + 2 * STAGES), bar_tempty = smem_u32(bars + 2 * STAGES + 2);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
@@ -338,7 +341,24 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     // rows of the output on 32-byte boundaries: each thread stores its own; else they pass through shared memory
     const bool vec = p.width % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
     const bool pairs = p.width % 2 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 3) == 0;
-    uint32_t* stage_out = reinterpret_cast<uint32_t*>(smem + C::SMEM_DATA + 256) + (warp - 2) * 32 * STAGE_OUT_LD;
+    unsigned char* box = sOut + (warp - 2) * OUT_BOX_BYTES;
+    uint32_t* stage_out = reinterpret_cast<uint32_t*>(box);
+    // a row's 32 elements from column c0 (0 or 32) into the box, in the 128-byte swizzle that the tensor map undoes
+    auto box_put = [&](int c0, const uint32_t(&o)[16]) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<uint4*>(box + lane * 128 + (((c0 >> 3) + q) ^ (lane & 7)) * 16) =
+            make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+    };
+    auto box_open = [&]() {   // the previous box has left
+      if (lane == 0) tma_store_wait_read();
+      __syncwarp();
+    };
+    auto box_send = [&](int x, int y) {
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) tma_store_2d(&tmOut, smem_u32(box), x, y);
+    };
     const uint32_t acc_mask = d.kb > 0 ? 0xffffffffu : 0u;   // no live rows: the accumulator holds stale values
     while (ok && walk.step()) {
       const Tile tl = decode<FORM, CTA2>(p, d, walk.t, rank);
@@ -346,10 +366,19 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       const bool row_live = row < d.m;
       const int col_first = tl.nt * BN + half * (BN / 2);
       const int left = d.n - col_first;   // columns of this half tile that exist
-      float off = 0.f;
+      // dW sums over blocks of BK rows: of dz, the rows up to that boundary are wanted, as zeros behind the last live one
+      const int rows_wanted = EPI == EPI_PROB ? (d.m + BK - 1) / BK * BK : d.m;
+      const bool idle = tl.mt * BM + quad * 32 >= rows_wanted || left <= 0 && EPI == EPI_OUT;   // nothing for this warp
+      float off = 0.f, diff = 0.f;
       long long out_row = row;
-      int want = -1;                      // EPI_LSE: column of the row's target in this half tile
-      if (EPI == EPI_PROB && row_live) off = p.shift - p.lse2[row];
+      int want = -1;                      // column of the row's target in this half tile
+      if (EPI == EPI_PROB && row_live) {
+        off = p.shift - p.lse2[row];
+        if (p.tgt) {
+          want = p.tgt[row] - p.class0 - col_first;
+          diff = p.tdiff[row];
+        }
+      }
       if (EPI == EPI_OUT && row_live) out_row = p.row_map ? p.row_map[row] : (long long)p.class0 + row;
       if (EPI == EPI_LSE && p.tgt && row_live) want = p.tgt[row] - col_first;
       ok = mbar_wait(bar_tfull + 8 * buf, (tphase >> buf) & 1, abort_flag, p.status, 14);
@@ -387,6 +416,10 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         release();
         f(96, b);
       };
+      if (idle) {
+        release();
+        continue;
+      }
       if (EPI == EPI_LSE) {
         // the few targets in this half tile
         unsigned hits = __ballot_sync(0xffffffffu, want >= 0 && want < BN / 2);
@@ -424,8 +457,6 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         });
         if (row_live) p.part[(long long)(2 * tl.nt + half) * p.part_ld + row] = make_float2(m * p.c, s);
       } else if (EPI == EPI_PROB) {
-        // the piece's buffer has whole tiles: every row and column of this one is written, zeros behind the last live ones
-        T* dst = static_cast<T*>(p.dz) + row * p.dz_ld + col_first;
         const uint32_t keep = row_live ? 0xffffffffu : 0u;
         chunks([&](int c0, uint32_t(&r)[32]) {
           uint32_t o[16];
@@ -443,10 +474,14 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
               o[i] &= have >= 2 ? 0xffffffffu : (have == 1 ? 0x0000ffffu : 0u);
             }
           }
-#pragma unroll
-          for (int q = 0; q < 16; q += 8)
-            st_global_32B(dst + c0 + 2 * q, make_uint4(o[q], o[q + 1], o[q + 2], o[q + 3]),
-                          make_uint4(o[q + 4], o[q + 5], o[q + 6], o[q + 7]));
+          if ((c0 & 32) == 0) box_open();
+          box_put(c0 & 32, o);
+          if (c0 & 32) {
+            const int at = want - (c0 & 64);
+            if (at >= 0 && at < 64)   // the difference at the target, rounded once
+              *reinterpret_cast<T*>(box + lane * 128 + ((at >> 3) ^ (lane & 7)) * 16 + (at & 7) * 2) = Num<T>::from_f(diff);
+            box_send(col_first + (c0 & 64), tl.mt * BM + quad * 32);
+          }
         });
       } else if (walk.slot >= 0 || (ACC && p.acc_out)) {
         // float32 results: a part of a split tile, or the sums over the pieces so far (row strides of whole tiles: no bounds)
@@ -474,7 +509,7 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       } else {
         T* dst = static_cast<T*>(p.out) + out_row * p.width + col_first;
         chunks([&](int c0, uint32_t(&r)[32]) {
-          if (left <= c0) return;   // the same for the whole warp
+          if (left <= (c0 & 64)) return;   // the same for the whole warp
           uint32_t o[16];
           if (ACC) {
             const float* acc = p.acc + row * p.acc_ld + col_first + c0;
@@ -492,6 +527,12 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 #pragma unroll
           for (int i = 0; i < 32; i += 2)
             o[i >> 1] = pack_pair<T>(__uint_as_float(r[i] & acc_mask) * g, __uint_as_float(r[i + 1] & acc_mask) * g);
+          if (p.boxes) {
+            if ((c0 & 32) == 0) box_open();
+            box_put(c0 & 32, o);
+            if (c0 & 32) box_send(col_first + (c0 & 64), p.class0 + tl.mt * BM + quad * 32);
+            return;
+          }
           if (vec && left >= c0 + 32) {
             if (row_live) {
 #pragma unroll
@@ -501,6 +542,7 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             }
             return;
           }
+          if (left <= c0) return;
           // the warp's 32 x 32 block through shared memory, stored row by row in neighbouring lanes
 #pragma unroll
           for (int i = 0; i < 16; ++i) stage_out[lane * STAGE_OUT_LD + i] = o[i];
@@ -526,6 +568,7 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         });
       }
     }
+    if (lane == 0) tma_store_wait();   // the last boxes are in place before the kernel ends
   }
   // ---------------- teardown ----------------
   tc_fence_before();
@@ -651,8 +694,10 @@ __device__ __forceinline__ bool row_is_live(const long long* target, const int32
 __global__ void __launch_bounds__(kRowThreads)
 pack_rows_kernel(const uint16_t* __restrict__ hidden, long long ld, const long long* __restrict__ target, const int32_t* __restrict__ flags,
                  int rows, int vocab, int width, uint16_t* __restrict__ packed, int packed_ld, int32_t* __restrict__ origin,
-                 int32_t* __restrict__ tgt, int32_t* __restrict__ pos, float* __restrict__ loss_rows, float* __restrict__ lse_rows) {
+                 int32_t* __restrict__ tgt, int32_t* __restrict__ pos, float* __restrict__ loss_rows, float* __restrict__ lse_rows,
+                 int* __restrict__ done) {
   chain_enter();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *done = 0;   // blocks of the forward pass's last kernel that have ended
   __shared__ int s_warp[kRowThreads / 32];
   __shared__ int s_at[kRowThreads];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -699,8 +744,9 @@ pack_rows_kernel(const uint16_t* __restrict__ hidden, long long ld, const long l
 // blocks of BK rows: the last one is filled up with zeros (dz has zeros there, but 0 x NaN would remain).
 __global__ void __launch_bounds__(kRowThreads)
 repack_rows_kernel(const uint16_t* __restrict__ hidden, long long ld, const int32_t* __restrict__ pos, const float* __restrict__ lse_rows,
-                   int rows, int width, uint16_t* __restrict__ packed, int packed_ld, int32_t* __restrict__ origin, float* __restrict__ lse2,
-                   uint16_t* __restrict__ dhidden) {
+                   const long long* __restrict__ target, const float* __restrict__ loss_rows, float unit, int rows, int width,
+                   uint16_t* __restrict__ packed, int packed_ld, int32_t* __restrict__ origin, float* __restrict__ lse2,
+                   int32_t* __restrict__ tgt, float* __restrict__ tdiff, uint16_t* __restrict__ dhidden) {
   chain_enter();
   const int lane = threadIdx.x & 31;
   const int warps = gridDim.x * (kRowThreads / 32);
@@ -712,6 +758,10 @@ repack_rows_kernel(const uint16_t* __restrict__ hidden, long long ld, const int3
       if (lane == 0) {
         origin[at] = r;
         lse2[at] = lse_rows[r] * kLog2e;
+        if (target) {
+          tgt[at] = (int)target[r];
+          tdiff[at] = expm1f(-loss_rows[r]) * unit;   // probability of the target less 1
+        }
       }
     } else if (dhidden) {
       copy_row(dhidden + (long long)r * width, nullptr, width);
@@ -768,7 +818,8 @@ finish_rows_kernel(const float2* __restrict__ part, long long part_ld, int n_par
                    const int32_t* __restrict__ origin, const T* __restrict__ packed, int packed_ld, const T* __restrict__ weight,
                    long long weight_ld, int width, const int32_t* __restrict__ tgt, const float* __restrict__ zt,
                    const int32_t* __restrict__ idx, const float* __restrict__ q, const float* __restrict__ cw, int k, float inv_t,
-                   float* __restrict__ loss_rows, float* __restrict__ lse_rows, float* __restrict__ diff) {
+                   float* __restrict__ loss_rows, float* __restrict__ lse_rows, float* __restrict__ diff, int rows, int* __restrict__ done,
+                   float* __restrict__ mean, float* __restrict__ inv_live) {
   chain_enter();
   constexpr int G = kFinishThreads / kRows, W = kFinishThreads / 32;
   constexpr int DOTS = 4;
@@ -777,8 +828,7 @@ finish_rows_kernel(const float2* __restrict__ part, long long part_ld, int n_par
   __shared__ float s_lse[kRows];
   const int n = *count;
   const int base = blockIdx.x * kRows;
-  if (base >= n) return;
-  const int live = min(kRows, n - base);
+  const int live = max(0, min(kRows, n - base));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rr = threadIdx.x % kRows, grp = threadIdx.x / kRows;
   float m = -1e38f, s = 0.f;
@@ -804,7 +854,7 @@ finish_rows_kernel(const float2* __restrict__ part, long long part_ld, int n_par
     s_s[warp][lane] = s;
   }
   __syncthreads();
-  if (threadIdx.x < live) {
+  if ((int)threadIdx.x < live) {
     m = s_m[0][threadIdx.x];
     s = s_s[0][threadIdx.x];
     for (int w = 1; w < W; ++w) merge(s_m[w][threadIdx.x], s_s[w][threadIdx.x]);
@@ -824,9 +874,8 @@ finish_rows_kernel(const float2* __restrict__ part, long long part_ld, int n_par
         lse_rows[r] = fixed;
       }
     }
-    return;
   }
-  const int per_row = (k + DOTS - 1) / DOTS;
+  const int per_row = idx ? (k + DOTS - 1) / DOTS : 0;
   for (int t = warp; t < live * per_row; t += W) {
     const int i = t / per_row, e0 = (t - i * per_row) * DOTS, c = base + i;
     const long long at = (long long)origin[c] * k;
@@ -848,8 +897,8 @@ finish_rows_kernel(const float2* __restrict__ part, long long part_ld, int n_par
       diff[at + e] = have >= 0 ? expf(lp) - cw[at + e] : 0.f;
     }
   }
-  __syncthreads();
-  for (int i = warp; i < live; i += W) {
+  if (idx) __syncthreads();
+  for (int i = warp; idx && i < live; i += W) {
     float sum = 0.f;
     for (int e = lane; e < k; e += 32) sum += s_terms[i * k + e];
 #pragma unroll
@@ -859,6 +908,26 @@ finish_rows_kernel(const float2* __restrict__ part, long long part_ld, int n_par
       loss_rows[r] = sum / (inv_t * inv_t);
       lse_rows[r] = s_lse[i];
     }
+  }  // the block that ends last takes the mean: all rows in one order, in 64 bits
+  __shared__ bool s_last;
+  __shared__ double s_sum[W];
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) s_last = atomicAdd(done, 1) == (int)gridDim.x - 1;
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  double sum = 0.0;
+  for (int r = threadIdx.x; r < rows; r += kFinishThreads) sum += (double)__ldcg(loss_rows + r);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (lane == 0) s_sum[warp] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < W; ++w) sum += s_sum[w];
+    const int div = n > 1 ? n : 1;
+    *mean = (float)(sum / div);
+    *inv_live = 1.0f / (float)div;
   }
 }
 
@@ -882,22 +951,19 @@ teacher_kernel(const void* __restrict__ values, int vdtype, const long long* __r
   }
 }
 
-// dz at the targets of the piece: the difference in float32, rounded once.  Entries of one row that name the same class write the same value.
+// dz at the teacher's classes of the piece: the difference in float32, rounded once.  Entries of one row that name the same class write the
+// same value.
 template <typename T>
 __global__ void __launch_bounds__(256)
-place_targets_kernel(const int32_t* __restrict__ count, const int32_t* __restrict__ origin, const long long* __restrict__ target,
-                     const float* __restrict__ loss_rows, const long long* __restrict__ top_indices, const float* __restrict__ diff, int k,
-                     int class0, int classes, float unit, T* __restrict__ dz, long long dz_ld) {
+place_targets_kernel(const int32_t* __restrict__ count, const int32_t* __restrict__ origin, const long long* __restrict__ top_indices,
+                     const float* __restrict__ diff, int k, int class0, int classes, float unit, T* __restrict__ dz, long long dz_ld) {
   chain_enter();
   const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   const long long c = i / k;
   if (c >= *count) return;
-  const long long r = origin[c];
-  const long long e = r * k + (i - c * k);
-  const long long at = (target ? target[r] : top_indices[e]) - class0;
-  if (at < 0 || at >= classes) return;
-  const float v = target ? expm1f(-loss_rows[r]) : diff[e];
-  dz[c * dz_ld + at] = Num<T>::from_f(v * unit);
+  const long long e = (long long)origin[c] * k + (i - c * k);
+  const long long at = top_indices[e] - class0;
+  if (at >= 0 && at < classes) dz[c * dz_ld + at] = Num<T>::from_f(diff[e] * unit);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
@@ -919,7 +985,7 @@ static int make_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t 
 static bool paired_for(int m) { return m > BM; }
 
 template <typename T, int FORM, int EPI, bool CTA2, bool ACC>
-static int launch_form(const CUtensorMap& tmA, const CUtensorMap& tmB, const Params& p, long long units, bool split, int* workers,
+static int launch_form(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut, const Params& p, long long units, bool split, int* workers,
                        cudaStream_t st) {
   auto kernel = head_product_kernel<T, FORM, EPI, CTA2, ACC>;
   constexpr int SMEM = Cfg<CTA2>::SMEM_BYTES;
@@ -952,13 +1018,13 @@ static int launch_form(const CUtensorMap& tmA, const CUtensorMap& tmB, const Par
   cfg.numAttrs = CTA2 ? 2 : 1;
   {
     ProfScope prof("head_product_kernel", st);
-    cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, p);
+    cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, tmOut, p);
   }
   return launch_status("head_product_kernel");
 }
 
 template <typename T, int FORM, int EPI, bool CTA2>
-static int launch_product_as(const CUtensorMap& tmA, const CUtensorMap& tmB, const Params& p, int m, int n, int k, cudaStream_t st) {
+static int launch_product_as(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut, const Params& p, int m, int n, int k, cudaStream_t st) {
   constexpr int UNIT = CTA2 ? 2 * BM : BM;
   const long long units = ((long long)(m + UNIT - 1) / UNIT) * ((n + BN - 1) / BN);
   LANCET_REQUIRE(units < (1ll << 30), LANCET_ERR_INVALID, "head product: %lld tiles", units);
@@ -966,11 +1032,11 @@ static int launch_product_as(const CUtensorMap& tmA, const CUtensorMap& tmB, con
   int workers = 0;
   if constexpr (FORM == FORM_DH) {
     if (p.acc) {
-      if (int rc = launch_form<T, FORM, EPI, CTA2, true>(tmA, tmB, p, units, split, &workers, st)) return rc;
-    } else if (int rc = launch_form<T, FORM, EPI, CTA2, false>(tmA, tmB, p, units, split, &workers, st)) {
+      if (int rc = launch_form<T, FORM, EPI, CTA2, true>(tmA, tmB, tmOut, p, units, split, &workers, st)) return rc;
+    } else if (int rc = launch_form<T, FORM, EPI, CTA2, false>(tmA, tmB, tmOut, p, units, split, &workers, st)) {
       return rc;
     }
-  } else if (int rc = launch_form<T, FORM, EPI, CTA2, false>(tmA, tmB, p, units, split, &workers, st)) {
+  } else if (int rc = launch_form<T, FORM, EPI, CTA2, false>(tmA, tmB, tmOut, p, units, split, &workers, st)) {
     return rc;
   }
   if constexpr (EPI == EPI_OUT) {
@@ -985,9 +1051,9 @@ static int launch_product_as(const CUtensorMap& tmA, const CUtensorMap& tmB, con
 }
 // m, n, k: upper bounds of the product's sizes (the live rows are known on the device only)
 template <typename T, int FORM, int EPI>
-static int launch_product(const CUtensorMap& tmA, const CUtensorMap& tmB, const Params& p, int m, int n, int k, bool paired, cudaStream_t st) {
-  return paired ? launch_product_as<T, FORM, EPI, true>(tmA, tmB, p, m, n, k, st)
-                : launch_product_as<T, FORM, EPI, false>(tmA, tmB, p, m, n, k, st);
+static int launch_product(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut, const Params& p, int m, int n, int k, bool paired, cudaStream_t st) {
+  return paired ? launch_product_as<T, FORM, EPI, true>(tmA, tmB, tmOut, p, m, n, k, st)
+                : launch_product_as<T, FORM, EPI, false>(tmA, tmB, tmOut, p, m, n, k, st);
 }
 
 struct Carver {
@@ -1012,6 +1078,7 @@ struct FwdWs {
   int32_t* origin;
   float2* part;
   int32_t* tgt;
+  int* done;
   float* zt;
   float* q;
   float* cw;
@@ -1027,6 +1094,7 @@ static FwdWs fwd_ws(void* ws, int rows, int vocab, int width, int k) {
   w.part = c.take<float2>((size_t)2 * ((vocab + BN - 1) / BN) * pad_rows(rows));
   w.tgt = c.take<int32_t>(k ? 0 : rows);
   w.zt = c.take<float>(k ? 0 : rows);
+  w.done = c.take<int>(1);
   w.q = c.take<float>((size_t)rows * k);
   w.cw = c.take<float>((size_t)rows * k);
   w.idx = c.take<int32_t>((size_t)rows * k);
@@ -1052,6 +1120,8 @@ struct BwdWs {
   uint16_t* packed;
   int32_t* origin;
   float* lse2;
+  int32_t* tgt;
+  float* tdiff;
   uint16_t* dz;
   float* acc;
   float* slots;
@@ -1065,6 +1135,8 @@ static BwdWs bwd_ws(void* ws, int rows, int vocab, int width) {
   w.packed = c.take<uint16_t>((size_t)pad_rows(rows) * pad_width(width));
   w.origin = c.take<int32_t>(rows);
   w.lse2 = c.take<float>(pad_rows(rows));
+  w.tgt = c.take<int32_t>(rows);
+  w.tdiff = c.take<float>(rows);
   w.dz = c.take<uint16_t>((size_t)pad_rows(rows) * w.piece);
   w.acc = c.take<float>(w.piece < vocab ? (size_t)pad_rows(rows) * pad_cols(width) : 0);
   const bool split = (w.piece < vocab ? w.piece : vocab) > SPLIT_MIN_KB * BK || rows > SPLIT_MIN_KB * BK;
@@ -1123,7 +1195,7 @@ static int finish_launch(const FwdArgs& a, const FwdWs& w, int n_part, cudaStrea
                    static_cast<const float2*>(w.part), pad_rows(a.rows), n_part, static_cast<const int32_t*>(a.pos + a.rows),
                    static_cast<const int32_t*>(w.origin), packed, pad_width(a.width), weight, a.ldw, a.width,
                    static_cast<const int32_t*>(w.tgt), static_cast<const float*>(w.zt), static_cast<const int32_t*>(a.target ? nullptr : w.idx), static_cast<const float*>(w.q), static_cast<const float*>(w.cw), a.k, a.inv_t,
-                   a.loss_rows, a.lse_rows, a.diff);
+                   a.loss_rows, a.lse_rows, a.diff, a.rows, w.done, a.mean, a.inv_live);
     return launch_status("finish_rows_kernel");
   };
   // 8 rows a block read the partial sums in whole sectors; with few rows, more blocks
@@ -1145,7 +1217,7 @@ static int linear_fwd(const char* fn, const FwdArgs& a, cudaStream_t st) {
   blocks = blocks > 4 * 148 ? 4 * 148 : blocks;
   launch_chained(pack_rows_kernel, dim3(blocks), dim3(kRowThreads), 0, st, static_cast<const uint16_t*>(a.hidden), a.ldh, a.target,
                  static_cast<const int32_t*>(a.target ? nullptr : w.live), a.rows, a.vocab, a.width, w.packed, pad_width(a.width), w.origin,
-                 w.tgt, a.pos, a.loss_rows, a.lse_rows);
+                 w.tgt, a.pos, a.loss_rows, a.lse_rows, w.done);
   if (int rc = launch_status("pack_rows_kernel")) return rc;
   const bool paired = paired_for(a.rows);
   CUtensorMap tmA, tmB;
@@ -1161,13 +1233,11 @@ static int linear_fwd(const char* fn, const FwdArgs& a, cudaStream_t st) {
   p.part_ld = pad_rows(a.rows);
   p.tgt = a.target ? w.tgt : nullptr;
   p.zt = w.zt;
-  int rc = a.dtype == LANCET_BF16 ? launch_product<__nv_bfloat16, FORM_Z, EPI_LSE>(tmA, tmB, p, a.rows, a.vocab, a.width, paired, st)
-                                  : launch_product<__half, FORM_Z, EPI_LSE>(tmA, tmB, p, a.rows, a.vocab, a.width, paired, st);
+  int rc = a.dtype == LANCET_BF16 ? launch_product<__nv_bfloat16, FORM_Z, EPI_LSE>(tmA, tmB, tmA, p, a.rows, a.vocab, a.width, paired, st)
+                                  : launch_product<__half, FORM_Z, EPI_LSE>(tmA, tmB, tmA, p, a.rows, a.vocab, a.width, paired, st);
   if (rc) return rc;
   const int n_part = 2 * ((a.vocab + BN - 1) / BN);
-  rc = a.dtype == LANCET_BF16 ? finish_launch<__nv_bfloat16>(a, w, n_part, st) : finish_launch<__half>(a, w, n_part, st);
-  if (rc) return rc;
-  return launch_mean(a.loss_rows, nullptr, a.pos + a.rows, a.rows, a.mean, a.inv_live, st);
+  return a.dtype == LANCET_BF16 ? finish_launch<__nv_bfloat16>(a, w, n_part, st) : finish_launch<__half>(a, w, n_part, st);
 }
 
 struct BwdArgs {
@@ -1195,17 +1265,18 @@ struct BwdArgs {
 
 template <typename T>
 static int linear_bwd_t(const BwdArgs& a, const BwdWs& w, cudaStream_t st) {
-  int blocks = (a.rows + 7) / 8;
-  blocks = blocks > 4 * 148 ? 4 * 148 : (blocks < 8 ? 8 : blocks);   // the zero rows want some warps even for one row
-  launch_chained(repack_rows_kernel, dim3(blocks), dim3(kRowThreads), 0, st, static_cast<const uint16_t*>(a.hidden), a.ldh, a.pos, a.lse_rows,
-                 a.rows, a.width, w.packed, pad_width(a.width), w.origin, w.lse2, static_cast<uint16_t*>(a.dhidden));
-  if (int rc = launch_status("repack_rows_kernel")) return rc;
-  const bool paired = paired_for(a.rows);
-  const long long padded = pad_rows(a.rows);
   // dz is kept in 16 bits.  In float16 it carries a factor of 2^14 (its values are within [-1, 1]): probabilities down to 2^-38 keep their
   // 11 bits instead of vanishing below 2^-24; the factor leaves again in the products' float32 results.
   const float shift = a.dtype == LANCET_F16 ? 14.f : 0.f;
   const float unit = a.dtype == LANCET_F16 ? 16384.f : 1.f;
+  int blocks = (a.rows + 7) / 8;
+  blocks = blocks > 4 * 148 ? 4 * 148 : (blocks < 8 ? 8 : blocks);   // the zero rows want some warps even for one row
+  launch_chained(repack_rows_kernel, dim3(blocks), dim3(kRowThreads), 0, st, static_cast<const uint16_t*>(a.hidden), a.ldh, a.pos, a.lse_rows,
+                 a.target, a.loss_rows, unit, a.rows, a.width, w.packed, pad_width(a.width), w.origin, w.lse2, w.tgt, w.tdiff,
+                 static_cast<uint16_t*>(a.dhidden));
+  if (int rc = launch_status("repack_rows_kernel")) return rc;
+  const bool paired = paired_for(a.rows);
+  const long long padded = pad_rows(a.rows);
   Params p = {};
   p.count = a.pos + a.rows;
   p.width = a.width;
@@ -1213,30 +1284,37 @@ static int linear_bwd_t(const BwdArgs& a, const BwdWs& w, cudaStream_t st) {
   p.c = a.inv_t * kLog2e;
   p.lse2 = w.lse2;
   p.shift = shift;
-  p.dz = w.dz;
-  p.dz_ld = w.piece;
+  p.tgt = a.target ? w.tgt : nullptr;
+  p.tdiff = w.tdiff;
   p.grad_out = a.grad_out;
   p.inv_live = a.inv_live;
   p.slots = w.slots;
   p.scale = a.scale / (a.inv_t * unit);
-  CUtensorMap hK, wK, dzK, wMN, dzMN, hMN;
+  CUtensorMap hK, wK, dzK, wMN, dzMN, hMN, dzOut, dwOut;
   if (int rc = make_map(&hK, w.packed, padded, a.width, pad_width(a.width), BM, a.dtype)) return rc;
   if (int rc = make_map(&wK, a.weight, a.vocab, a.width, a.ldw, paired ? BN / 2 : BN, a.dtype)) return rc;
   if (int rc = make_map(&dzK, w.dz, padded, w.piece, w.piece, BM, a.dtype)) return rc;
   if (int rc = make_map(&wMN, a.weight, a.vocab, a.width, a.ldw, 64, a.dtype)) return rc;
   if (int rc = make_map(&dzMN, w.dz, padded, w.piece, w.piece, 64, a.dtype)) return rc;
+  if (int rc = make_map(&dzOut, w.dz, padded, w.piece, w.piece, OUT_BOX_ROWS, a.dtype)) return rc;
+  const bool boxes = a.dweight && a.width % 8 == 0 && aligned(a.dweight, 16);
+  dwOut = dzOut;
+  if (boxes)   // rows behind the vocabulary are no part of it
+    if (int rc = make_map(&dwOut, a.dweight, a.vocab, a.width, a.width, OUT_BOX_ROWS, a.dtype)) return rc;
   if (int rc = make_map(&hMN, w.packed, padded, a.width, pad_width(a.width), 64, a.dtype)) return rc;
   for (int v0 = 0; v0 < a.vocab; v0 += w.piece) {
     const int classes = a.vocab - v0 < w.piece ? a.vocab - v0 : w.piece;
     const bool last = v0 + classes == a.vocab;
     p.class0 = v0;
     p.classes = classes;
-    if (int rc = launch_product<T, FORM_Z, EPI_PROB>(hK, wK, p, a.rows, classes, a.width, paired, st)) return rc;
-    const long long entries = (long long)a.rows * a.k;
-    launch_chained(place_targets_kernel<T>, dim3((unsigned)((entries + 255) / 256)), dim3(256), 0, st, static_cast<const int32_t*>(p.count),
-                   static_cast<const int32_t*>(w.origin), a.target, a.loss_rows, a.indices, a.diff, a.k, v0, classes, unit,
-                   reinterpret_cast<T*>(w.dz), (long long)w.piece);
-    if (int rc = launch_status("place_targets_kernel")) return rc;
+    if (int rc = launch_product<T, FORM_Z, EPI_PROB>(hK, wK, dzOut, p, a.rows, classes, a.width, paired, st)) return rc;
+    if (!a.target) {
+      const long long entries = (long long)a.rows * a.k;
+      launch_chained(place_targets_kernel<T>, dim3((unsigned)((entries + 255) / 256)), dim3(256), 0, st, static_cast<const int32_t*>(p.count),
+                     static_cast<const int32_t*>(w.origin), a.indices, a.diff, a.k, v0, classes, unit, reinterpret_cast<T*>(w.dz),
+                     (long long)w.piece);
+      if (int rc = launch_status("place_targets_kernel")) return rc;
+    }
     Params ph = p;
     ph.out = a.dhidden;
     ph.row_map = w.origin;
@@ -1247,11 +1325,12 @@ static int linear_bwd_t(const BwdArgs& a, const BwdWs& w, cudaStream_t st) {
       ph.acc_out = !last;
     }
     if (a.dhidden)
-      if (int rc = launch_product<T, FORM_DH, EPI_OUT>(dzK, wMN, ph, a.rows, a.width, classes, paired, st)) return rc;
+      if (int rc = launch_product<T, FORM_DH, EPI_OUT>(dzK, wMN, dzK, ph, a.rows, a.width, classes, paired, st)) return rc;
     if (!a.dweight) continue;
     Params pw = p;
     pw.out = a.dweight;
-    if (int rc = launch_product<T, FORM_DW, EPI_OUT>(dzMN, hMN, pw, classes, a.width, a.rows, paired_for(classes), st)) return rc;
+    pw.boxes = boxes;
+    if (int rc = launch_product<T, FORM_DW, EPI_OUT>(dzMN, hMN, dwOut, pw, classes, a.width, a.rows, paired_for(classes), st)) return rc;
   }
   return LANCET_OK;
 }

@@ -457,8 +457,10 @@ int lancet_softmax_xent_bwd(const void* logits, long long ld, const long long* t
  * pos [rows + 1] int32: packed index of every row that takes part or -1, then their number; diff [rows][k] float32: student minus teacher
  * probability at the teacher's classes; the backward calls take both.  mean = sum(loss_rows) * inv_live, inv_live = 1 / max(live rows, 1)
  * (float32 scalars on the device).
+ * lancet_copy_rows: rows of 16-bit elements to a destination with 16-byte aligned rows (ldd % 8 == 0), for a weight that has none.
  * ws: lancet_linear_loss_*_workspace_bytes bytes (k = 0 for the cross entropy), 256-byte aligned, used by this call only.  status: int32 on
  * the device, as for the grouped GEMM. */
+int lancet_copy_rows(const void* src, long long lds, void* dst, long long ldd, int rows, int width, lancet_stream_t stream);
 size_t lancet_linear_loss_fwd_workspace_bytes(int rows, int vocab, int width, int k);
 size_t lancet_linear_loss_bwd_workspace_bytes(int rows, int vocab, int width);
 int lancet_linear_xent_fwd(const void* hidden, long long ldh, const void* weight, long long ldw, const long long* target, int rows, int vocab,

@@ -164,6 +164,7 @@ SIGNATURES = {
     "lancet_softmax_xent_fwd": (c_int, [c_void_p, ctypes.c_longlong, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "lancet_softmax_xent_bwd": (c_int, [c_void_p, ctypes.c_longlong, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
                                         ctypes.c_float, c_void_p, ctypes.c_longlong, c_void_p]),
+    "lancet_copy_rows": (c_int, [c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_longlong, c_int, c_int, c_void_p]),
     "lancet_linear_loss_fwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "lancet_linear_loss_bwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "lancet_linear_xent_fwd": (c_int, [c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_longlong, c_void_p, c_int, c_int,

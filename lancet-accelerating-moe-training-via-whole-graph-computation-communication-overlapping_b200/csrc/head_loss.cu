@@ -23,8 +23,6 @@ using namespace lancet::gemm;
 constexpr int BM = 128, BN = 256, BK = 64, UMMA_K = 16;
 constexpr int A_STAGE_BYTES = BM * BK * 2;
 constexpr int EPI_WARPS = 8;
-constexpr int OUT_BOX_ROWS = 32, OUT_BOX_BYTES = OUT_BOX_ROWS * 128;   // an epilogue warp's box on its way out: 32 rows x 64 16-bit elements
-constexpr int STAGE_OUT_LD = 17;                // words of a staged row where rows go out singly: 32 elements and one word against bank conflicts
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int TMEM_COLS = 512;
 constexpr int ROW_PAD = 256;                    // row buffers hold a multiple of this: whole tiles, in the paired form too
@@ -37,14 +35,20 @@ constexpr long long BAND_BYTES = 20ll << 20;    // rows of A swept against all c
 constexpr int FORM_Z = 0, FORM_DH = 1, FORM_DW = 2;
 constexpr int EPI_LSE = 0, EPI_PROB = 1, EPI_OUT = 2;
 
-template <bool CTA2>
+// Boxes of 16-bit results on their way out, 32 rows x 64 columns in the 128-byte swizzle: two per epilogue warp where whole tiles leave this way
+// (one is filled while the other leaves), none for the row sums.  The operand stages take what is left of the shared memory.
+constexpr int OUT_ROWS = 32, OUT_COLS = BK, OUT_BOX_BYTES = OUT_ROWS * OUT_COLS * 2;
+constexpr int SMEM_MOST = 227 * 1024, SMEM_SLACK = 1024 /*alignment*/ + 256 /*barriers*/;
+template <int FORM, int EPI, bool CTA2>
 struct Cfg {
-  static constexpr int STAGES = CTA2 ? 6 : 4;
+  static constexpr int OUT_BYTES = EPI_WARPS * OUT_BOX_BYTES * (EPI == EPI_LSE ? 0 : FORM == FORM_DH ? 1 : 2);
   static constexpr int B_COLS = CTA2 ? BN / 2 : BN;
   static constexpr int B_STAGE_BYTES = B_COLS * BK * 2;
   static constexpr int STAGE_BYTES = A_STAGE_BYTES + B_STAGE_BYTES;
+  static constexpr int FIT = (SMEM_MOST - SMEM_SLACK - OUT_BYTES) / STAGE_BYTES;
+  static constexpr int STAGES = FIT > 6 ? 6 : FIT;
   static constexpr int SMEM_DATA = STAGES * STAGE_BYTES;
-  static constexpr int SMEM_BYTES = SMEM_DATA + EPI_WARPS * OUT_BOX_BYTES + 1024 /*alignment slack*/ + 256 /*barriers*/;
+  static constexpr int SMEM_BYTES = SMEM_DATA + OUT_BYTES + SMEM_SLACK;
 };
 
 struct Params {
@@ -208,15 +212,15 @@ template <typename T, int FORM, int EPI, bool CTA2, bool ACC>
 __global__ void __launch_bounds__(THREADS, 1)
 head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmOut,
                     Params p) {
-  using C = Cfg<CTA2>;
+  using C = Cfg<FORM, EPI, CTA2>;
   constexpr int STAGES = C::STAGES;
   constexpr bool A_MN = FORM == FORM_DW, B_MN = FORM != FORM_Z;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* sA = smem;
   unsigned char* sB = smem + STAGES * A_STAGE_BYTES;
-  unsigned char* sOut = smem + C::SMEM_DATA;   // a box per epilogue warp
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sOut + EPI_WARPS * OUT_BOX_BYTES);
+  unsigned char* sOut = smem + C::SMEM_DATA;   // the epilogue warps' boxes
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sOut + C::OUT_BYTES);
   const uint32_t bar_full = smem_u32(bars), bar_empty = smem_u32(bars + STAGES);
   const uint32_t bar_tfull = smem_u32(bars + 2 * STAGES), bar_tempty = smem_u32(bars + 2 * STAGES + 2);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
@@ -340,24 +344,25 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     if (EPI == EPI_OUT) g = p.scale * (p.grad_out ? *p.grad_out : 1.f) * (p.inv_live ? *p.inv_live : 1.f);
     // rows of the output on 32-byte boundaries: each thread stores its own; else they pass through shared memory
     const bool vec = p.width % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
-    const bool pairs = p.width % 2 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 3) == 0;
-    unsigned char* box = sOut + (warp - 2) * OUT_BOX_BYTES;
-    uint32_t* stage_out = reinterpret_cast<uint32_t*>(box);
-    // a row's 32 elements from column c0 (0 or 32) into the box, in the 128-byte swizzle that the tensor map undoes
-    auto box_put = [&](int c0, const uint32_t(&o)[16]) {
+    constexpr int BOXES = C::OUT_BYTES / (EPI_WARPS * OUT_BOX_BYTES);
+    unsigned char* boxes = sOut + (warp - 2) * BOXES * OUT_BOX_BYTES;
+    int box_at = 0;
+    // 16-byte unit `unit` (of 8) of row r of the box in turn, where the tensor map's swizzle has it
+    auto box_unit = [&](int r, int unit) { return boxes + box_at + r * 128 + ((unit ^ (r & 7)) << 4); };
+    auto box_put = [&](int c0, const uint32_t(&o)[16]) {   // the lane's row, 32 elements from column c0 (0 or 32)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<uint4*>(box + lane * 128 + (((c0 >> 3) + q) ^ (lane & 7)) * 16) =
-            make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+        *reinterpret_cast<uint4*>(box_unit(lane, (c0 >> 3) + q)) = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
     };
-    auto box_open = [&]() {   // the previous box has left
-      if (lane == 0) tma_store_wait_read();
+    auto box_open = [&]() {   // the box before the last has left
+      if (lane == 0) tma_store_wait_read<1>();
       __syncwarp();
     };
     auto box_send = [&](int x, int y) {
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) tma_store_2d(&tmOut, smem_u32(box), x, y);
+      if (lane == 0) tma_store_2d(&tmOut, smem_u32(boxes + box_at), x, y);
+      box_at ^= OUT_BOX_BYTES;
     };
     const uint32_t acc_mask = d.kb > 0 ? 0xffffffffu : 0u;   // no live rows: the accumulator holds stale values
     while (ok && walk.step()) {
@@ -390,7 +395,7 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          if (CTA2) mbar_arrive_cluster(cluster_addr(bar_tempty + 8 * buf, 0)); else mbar_arrive(bar_tempty + 8 * buf);
+          if (CTA2) mbar_arrive_cluster_tmem(cluster_addr(bar_tempty + 8 * buf, 0)); else mbar_arrive(bar_tempty + 8 * buf);
         }
         tphase ^= 1u << buf;
         buf ^= 1;
@@ -474,12 +479,11 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
               o[i] &= have >= 2 ? 0xffffffffu : (have == 1 ? 0x0000ffffu : 0u);
             }
           }
-          if ((c0 & 32) == 0) box_open();
+          if (!(c0 & 32)) box_open();
           box_put(c0 & 32, o);
           if (c0 & 32) {
             const int at = want - (c0 & 64);
-            if (at >= 0 && at < 64)   // the difference at the target, rounded once
-              *reinterpret_cast<T*>(box + lane * 128 + ((at >> 3) ^ (lane & 7)) * 16 + (at & 7) * 2) = Num<T>::from_f(diff);
+            if (at >= 0 && at < 64) *reinterpret_cast<T*>(box_unit(lane, at >> 3) + (at & 7) * 2) = Num<T>::from_f(diff);   // rounded once
             box_send(col_first + (c0 & 64), tl.mt * BM + quad * 32);
           }
         });
@@ -528,12 +532,12 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           for (int i = 0; i < 32; i += 2)
             o[i >> 1] = pack_pair<T>(__uint_as_float(r[i] & acc_mask) * g, __uint_as_float(r[i + 1] & acc_mask) * g);
           if (p.boxes) {
-            if ((c0 & 32) == 0) box_open();
+            if (!(c0 & 32)) box_open();
             box_put(c0 & 32, o);
             if (c0 & 32) box_send(col_first + (c0 & 64), p.class0 + tl.mt * BM + quad * 32);
             return;
           }
-          if (vec && left >= c0 + 32) {
+          if (vec && left >= (c0 & 64) + 64) {
             if (row_live) {
 #pragma unroll
               for (int q = 0; q < 16; q += 8)
@@ -542,27 +546,26 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             }
             return;
           }
-          if (left <= c0) return;
-          // the warp's 32 x 32 block through shared memory, stored row by row in neighbouring lanes
-#pragma unroll
-          for (int i = 0; i < 16; ++i) stage_out[lane * STAGE_OUT_LD + i] = o[i];
+          // rows on other boundaries: the warp's 32 x 64 block through a box, then row by row in neighbouring lanes, 4 bytes each; a row
+          // that starts between 4-byte boundaries goes out as its first element, words across the staged ones, and its last element
+          box_put(c0 & 32, o);
+          if (!(c0 & 32)) return;
           __syncwarp();
-          const int cols = min(32, left - c0), rows = min(32, d.m - (tl.mt * BM + quad * 32));
-          const unsigned long long at = reinterpret_cast<unsigned long long>(dst + c0);
-          if (pairs) {
-            const int sub = lane >> 4, w = lane & 15;
-#pragma unroll 4
-            for (int i = 0; i < 32; i += 2) {
-              uint32_t* to = reinterpret_cast<uint32_t*>(__shfl_sync(0xffffffffu, at, i + sub));
-              if (i + sub < rows && 2 * w < cols) to[w] = stage_out[(i + sub) * STAGE_OUT_LD + w];   // an even width has even `cols`
-            }
-          } else {
-            const uint16_t* st = reinterpret_cast<const uint16_t*>(stage_out);
-#pragma unroll 4
-            for (int i = 0; i < 32; ++i) {
-              uint16_t* to = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, at, i));
-              if (i < rows && lane < cols) to[lane] = st[2 * i * STAGE_OUT_LD + lane];
-            }
+          const int cols = min(64, left - (c0 & 64)), rows = min(32, d.m - (tl.mt * BM + quad * 32));
+          const unsigned long long mine = reinterpret_cast<unsigned long long>(dst + (c0 & 64));
+          const unsigned long long first = __shfl_sync(0xffffffffu, mine, 0);
+#pragma unroll 8
+          for (int r = 0; r < 32; ++r) {
+            unsigned char* to = reinterpret_cast<unsigned char*>(p.row_map ? __shfl_sync(0xffffffffu, mine, r)
+                                                                           : first + (unsigned long long)(2 * r) * p.width);
+            const uint32_t word = *reinterpret_cast<const uint32_t*>(box_unit(r, lane >> 2) + (lane & 3) * 4);
+            const uint32_t next = __shfl_down_sync(0xffffffffu, word, 1);
+            const int odd = (reinterpret_cast<uintptr_t>(to) >> 1) & 1;      // elements before the first 4-byte boundary
+            const uint32_t out = odd ? __funnelshift_r(word, next, 16) : word;
+            const int e = r < rows ? 2 * lane + odd : 64;                    // first of this lane's two elements
+            if (e == 1 && lane == 0) *reinterpret_cast<uint16_t*>(to) = (uint16_t)word;
+            if (e + 1 < cols) *reinterpret_cast<uint32_t*>(to + 2 * e) = out;
+            if (e + 1 == cols) *reinterpret_cast<uint16_t*>(to + 2 * e) = (uint16_t)out;
           }
           __syncwarp();
         });
@@ -590,40 +593,49 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
 }
 
-// Adds the parts of split tiles in a fixed order and finishes them as the product's epilogue does.  A block takes JOIN_ROWS rows of a tile, a
-// thread four columns; where a tile has many parts (few rows), the block's four groups of threads share the parts of one row, else each group has
-// a row of its own.
-constexpr int JOIN_ROWS = 4, JOIN_SHARED_PARTS = 8;
+// Adds the parts of split tiles in a fixed order and finishes them as the product's epilogue does; a thread takes four columns.  Where tiles have
+// many parts (few rows) a block takes one row and its four groups of threads share the parts, else each group has a row of its own.
+constexpr int JOIN_ROWS = 4, JOIN_MANY = 8;
+struct JoinTile {
+  int mu, nt, w0, w1, late;   // unit, column tile; first and last worker with a part; whether the first one's is its second part
+};
 template <typename T, int FORM, bool CTA2>
-__global__ void __launch_bounds__(256) join_tiles_kernel(Params p, int workers) {
+__global__ void __launch_bounds__(256) join_tiles_kernel(Params p, int workers, int rows_per_block) {
   chain_enter();
   __shared__ float4 s_part[4][64];
+  __shared__ JoinTile s_tile;
   const Dims d = dims_of<FORM, CTA2>(p);
-  const Split s = split_of(d.mu * d.nt, d.kb, workers);
-  const int j = blockIdx.x;
-  if (j >= s.rem) return;
-  int mu, nt;
-  decode_unit<FORM, CTA2>(p, d, s.full + j, mu, nt);
+  if (threadIdx.x == 0) {
+    const Split s = split_of(d.mu * d.nt, d.kb, workers);
+    JoinTile jt = {0, 0, 0, -1, 0};   // no parts
+    const int j = blockIdx.x;
+    if (j < s.rem) {
+      decode_unit<FORM, CTA2>(p, d, s.full + j, jt.mu, jt.nt);
+      const long long a = (long long)j * s.kb, b = a + s.kb;
+      jt.w0 = (int)(a * s.parts / s.iters);
+      while (jt.w0 > 0 && s.begin(jt.w0) > a) --jt.w0;
+      while (s.begin(jt.w0 + 1) <= a) ++jt.w0;
+      jt.w1 = (int)((b - 1) * s.parts / s.iters);
+      while (jt.w1 > 0 && s.begin(jt.w1) > b - 1) --jt.w1;
+      while (s.begin(jt.w1 + 1) <= b - 1) ++jt.w1;
+      jt.late = s.begin(jt.w0) < a;
+      if (jt.w0 == jt.w1 && !jt.late && s.begin(jt.w0 + 1) == b) jt.w1 = -1;   // one worker had all of it
+    }
+    s_tile = jt;
+  }
+  __syncthreads();
+  const JoinTile jt = s_tile;
   constexpr int UNIT = CTA2 ? 2 * BM : BM;
-  const int row0 = blockIdx.y * JOIN_ROWS;
-  if (mu * UNIT + row0 >= d.m) return;
-  const long long a = (long long)j * s.kb, b = a + s.kb;
-  int w0 = (int)(a * s.parts / s.iters), w1;
-  while (w0 > 0 && s.begin(w0) > a) --w0;
-  while (s.begin(w0 + 1) <= a) ++w0;
-  w1 = (int)((b - 1) * s.parts / s.iters);   // the worker that has the last block
-  while (w1 > 0 && s.begin(w1) > b - 1) --w1;
-  while (s.begin(w1 + 1) <= b - 1) ++w1;
-  const bool late = s.begin(w0) < a;         // the first worker began in the tile before: this is its second part
-  if (w0 == w1 && !late && s.begin(w0 + 1) == b) return;   // one worker had all of it
+  const int row0 = blockIdx.y * rows_per_block;
+  if (jt.w1 < 0 || jt.mu * UNIT + row0 >= d.m) return;
   const float g = p.scale * (p.grad_out ? *p.grad_out : 1.f) * (p.inv_live ? *p.inv_live : 1.f);
   const int col = (threadIdx.x & 63) * 4, grp = threadIdx.x >> 6;
-  const int n0 = nt * BN + col;
+  const int n0 = jt.nt * BN + col;
   auto sum = [&](int i, int from, int step) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int w = from; w <= w1; w += step) {
-      const int slot = 2 * w + (w == w0 && late ? 1 : 0);
+#pragma unroll 8
+    for (int w = from; w <= jt.w1; w += step) {
+      const int slot = 2 * w + (w == jt.w0 ? jt.late : 0);
       const float4 x = *reinterpret_cast<const float4*>(p.slots + ((long long)slot * UNIT + i) * BN + col);
       v.x += x.x;
       v.y += x.y;
@@ -633,7 +645,7 @@ __global__ void __launch_bounds__(256) join_tiles_kernel(Params p, int workers) 
     return v;
   };
   auto finish = [&](int i, const float4& x) {
-    const int row = mu * UNIT + i;
+    const int row = jt.mu * UNIT + i;
     const float v[4] = {x.x, x.y, x.z, x.w};
     float* acc = p.acc + row * p.acc_ld + n0;
     T* out = static_cast<T*>(p.out) + (p.row_map ? p.row_map[row] : (long long)p.class0 + row) * p.width + n0;
@@ -647,40 +659,67 @@ __global__ void __launch_bounds__(256) join_tiles_kernel(Params p, int workers) 
         out[c] = Num<T>::from_f(t * g);
     }
   };
-  if (w1 - w0 < JOIN_SHARED_PARTS) {
+  if (rows_per_block == JOIN_ROWS) {
     const int i = row0 + grp;
-    if (mu * UNIT + i < d.m) finish(i, sum(i, w0, 1));
-  } else {
-    for (int i = row0; i < row0 + JOIN_ROWS && mu * UNIT + i < d.m; ++i) {
-      s_part[grp][threadIdx.x & 63] = sum(i, w0 + grp, 4);
-      __syncthreads();
-      if (grp == 0) {
-        float4 v = s_part[0][threadIdx.x];
-        for (int o = 1; o < 4; ++o) {
-          const float4 x = s_part[o][threadIdx.x];
-          v.x += x.x;
-          v.y += x.y;
-          v.z += x.z;
-          v.w += x.w;
-        }
-        finish(i, v);
-      }
-      __syncthreads();
+    if (jt.mu * UNIT + i < d.m) finish(i, sum(i, jt.w0, 1));
+    return;
+  }
+  s_part[grp][threadIdx.x & 63] = sum(row0, jt.w0 + grp, 4);
+  __syncthreads();
+  if (grp == 0) {
+    float4 v = s_part[0][threadIdx.x];
+    for (int q = 1; q < 4; ++q) {
+      const float4 x = s_part[q][threadIdx.x];
+      v.x += x.x;
+      v.y += x.y;
+      v.z += x.z;
+      v.w += x.w;
     }
+    finish(row0, v);
   }
 }
 
 // ---- live rows ------------------------------------------------------------------------------------------------------------
 constexpr int kRowThreads = 256;
 
-// One row of 16-bit elements by one warp, 16 bytes a lane where both ends allow it.  src null: zeros.
-__device__ __forceinline__ void copy_row(uint16_t* dst, const uint16_t* src, int width) {
+// One row of 16-bit elements by one warp to a destination on a 16-byte boundary: 16 bytes a lane where the source allows it, else 4-byte words,
+// put together from two where the source lies between 4-byte boundaries.
+__device__ __forceinline__ void copy_row(uint16_t* __restrict__ dst, const uint16_t* __restrict__ src, int width) {
   const int lane = threadIdx.x & 31;
-  const bool vec = ((reinterpret_cast<uintptr_t>(dst) | reinterpret_cast<uintptr_t>(src)) & 15) == 0;
-  const int nv = vec ? width / 8 : 0;
-  for (int i = lane; i < nv; i += 32)
-    reinterpret_cast<uint4*>(dst)[i] = src ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0);
-  for (int i = nv * 8 + lane; i < width; i += 32) dst[i] = src ? src[i] : (uint16_t)0;
+  int done = 0;
+  if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+    const int nv = width / 8;
+#pragma unroll 4
+    for (int i = lane; i < nv; i += 32) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
+    done = nv * 8;
+  } else {
+    const int off = (reinterpret_cast<uintptr_t>(src) >> 1) & 1;
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(src - off);
+    const int nw = (width - off) / 2;   // the last word read ends inside the row
+    constexpr int N = 8;
+    for (int i0 = lane; i0 < nw; i0 += 32 * N) {   // all loads of a round before its stores
+      uint32_t a[N], b[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        a[n] = i0 + 32 * n < nw ? words[i0 + 32 * n] : 0u;
+        b[n] = off && i0 + 32 * n < nw ? words[i0 + 32 * n + 1] : 0u;
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (i0 + 32 * n < nw) reinterpret_cast<uint32_t*>(dst)[i0 + 32 * n] = off ? __funnelshift_r(a[n], b[n], 16) : a[n];
+    }
+    done = nw * 2;
+  }
+  for (int i = done + lane; i < width; i += 32) dst[i] = src[i];
+}
+// Zeros for a row on any boundary.
+__device__ __forceinline__ void zero_row(uint16_t* dst, int width) {
+  const int lane = threadIdx.x & 31;
+  const int head = min(width, (int)(((16 - (reinterpret_cast<uintptr_t>(dst) & 15)) & 15) / 2));
+  const int nv = (width - head) / 8;
+  if (lane < head) dst[lane] = 0;
+  for (int i = lane; i < nv; i += 32) reinterpret_cast<uint4*>(dst + head)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = head + nv * 8 + lane; i < width; i += 32) dst[i] = 0;
 }
 
 __device__ __forceinline__ bool row_is_live(const long long* target, const int32_t* flags, int r, int vocab) {
@@ -740,6 +779,14 @@ pack_rows_kernel(const uint16_t* __restrict__ hidden, long long ld, const long l
   if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) pos[rows] = before;
 }
 
+// Rows to a padded row stride (a weight whose rows a tensor map cannot describe).
+__global__ void __launch_bounds__(kRowThreads)
+copy_rows_kernel(const uint16_t* __restrict__ src, long long lds, uint16_t* __restrict__ dst, long long ldd, int rows, int width) {
+  chain_enter();
+  const int warps = gridDim.x * (kRowThreads / 32);
+  for (int r = blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5); r < rows; r += warps) copy_row(dst + r * ldd, src + r * lds, width);
+}
+
 // The same packing in the backward pass, from pos; gradient rows of ignored rows are zeroed, lse goes to packed order and base 2.  dW sums over
 // blocks of BK rows: the last one is filled up with zeros (dz has zeros there, but 0 x NaN would remain).
 __global__ void __launch_bounds__(kRowThreads)
@@ -764,31 +811,31 @@ repack_rows_kernel(const uint16_t* __restrict__ hidden, long long ld, const int3
         }
       }
     } else if (dhidden) {
-      copy_row(dhidden + (long long)r * width, nullptr, width);
+      zero_row(dhidden + (long long)r * width, width);
     }
   }
   const int count = pos[rows], end = (count + BK - 1) / BK * BK;
-  for (int i = count + first; i < end; i += warps) copy_row(packed + (long long)i * packed_ld, nullptr, width);
+  for (int i = count + first; i < end; i += warps) zero_row(packed + (long long)i * packed_ld, width);
 }
 
 // ---- row results ----------------------------------------------------------------------------------------------------------
 constexpr int kFinishThreads = 256;
 
-// N dot products of row a with rows of b by one warp, their loads in flight together.  All rows start on 16-byte boundaries (packed rows; the
-// weight's rows as the tensor map wants them).
-template <typename T, int N>
-__device__ __forceinline__ void warp_dots(const T* a, const T* const* b, int width, float* out) {
-  const int lane = threadIdx.x & 31;
+// Dot product of two rows by LANES neighbouring lanes; all of them get it.  Both rows start on 16-byte boundaries (packed rows; the weight's rows
+// as the tensor map wants them).
+template <typename T, int LANES, int N>
+__device__ __forceinline__ void group_dots(const T* __restrict__ a, const T* const* b, int width, float* out) {
+  const int sub = threadIdx.x & (LANES - 1);
   float s[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) s[n] = 0.f;
   const int nv = width / 8;
-#pragma unroll 2
-  for (int i = lane; i < nv; i += 32) {
+#pragma unroll 4
+  for (int i = sub; i < nv; i += LANES) {
     const uint4 x = reinterpret_cast<const uint4*>(a)[i];
     uint4 y[N];
 #pragma unroll
-    for (int n = 0; n < N; ++n) y[n] = __ldg(reinterpret_cast<const uint4*>(b[n]) + i);
+    for (int n = 0; n < N; ++n) y[n] = reinterpret_cast<const uint4*>(b[n])[i];
     const T* xs = reinterpret_cast<const T*>(&x);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -797,40 +844,69 @@ __device__ __forceinline__ void warp_dots(const T* a, const T* const* b, int wid
       for (int j = 0; j < 8; ++j) s[n] = fmaf(Num<T>::to_f(xs[j]), Num<T>::to_f(ys[j]), s[n]);
     }
   }
-  for (int i = nv * 8 + lane; i < width; i += 32)
+  for (int i = nv * 8 + sub; i < width; i += LANES)
 #pragma unroll
     for (int n = 0; n < N; ++n) s[n] = fmaf(Num<T>::to_f(a[i]), Num<T>::to_f(b[n][i]), s[n]);
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1)
+  for (int d = LANES / 2; d > 0; d >>= 1)
 #pragma unroll
     for (int n = 0; n < N; ++n) s[n] += __shfl_xor_sync(0xffffffffu, s[n], d);
 #pragma unroll
   for (int n = 0; n < N; ++n) out[n] = s[n];
 }
 
-// A block finishes kRows packed rows: joins the partial maxima and sums of its rows' column half tiles (in a fixed order), then its warps
-// compute the logits at the rows' targets, or at the k entries of their teachers (idx [rows][k], -1: none), as float32 dot products.  The
-// tensor cores cut the sums of products short (measured: up to 1e-5 low at a logit of 12), which the loss would show where a target
-// holds most of the probability: its share of the row's sum is replaced by the dot product's.
-template <typename T, int kRows>
-__global__ void __launch_bounds__(kFinishThreads)
-finish_rows_kernel(const float2* __restrict__ part, long long part_ld, int n_part, const int32_t* __restrict__ count,
-                   const int32_t* __restrict__ origin, const T* __restrict__ packed, int packed_ld, const T* __restrict__ weight,
-                   long long weight_ld, int width, const int32_t* __restrict__ tgt, const float* __restrict__ zt,
-                   const int32_t* __restrict__ idx, const float* __restrict__ q, const float* __restrict__ cw, int k, float inv_t,
-                   float* __restrict__ loss_rows, float* __restrict__ lse_rows, float* __restrict__ diff, int rows, int* __restrict__ done,
-                   float* __restrict__ mean, float* __restrict__ inv_live) {
+struct FinishArgs {
+  const float2* part;      // [n_part][part_ld] maxima and sums of the column half tiles
+  long long part_ld;
+  int n_part;
+  const int32_t* count;
+  const int32_t* origin;
+  const void* packed;
+  int packed_ld;
+  const void* weight;
+  long long weight_ld;
+  int width;
+  const int32_t* tgt;      // targets and their logits from the product, by packed row
+  const float* zt;
+  const int32_t* idx;      // teachers: classes (-1: none), q, class weights, [rows][k]
+  const float* q;
+  const float* cw;
+  int k;
+  float inv_t;
+  float *loss_rows, *lse_rows, *diff;
+  double* block_sums;
+  int* done;
+  float *mean, *inv_live;
+};
+
+// A block finishes kRows packed rows: joins the partial maxima and sums of its rows' column half tiles (in a fixed order), and computes the
+// logits at the rows' targets, or at the entries of their teachers, as float32 dot products.  The tensor cores cut the sums of products short
+// (measured: up to 1e-5 low at a logit of 12), which the loss would show where a target holds most of the probability: its share of the
+// row's sum is replaced by the dot product's.  A target's dot product takes a warp and is under way before the sums are joined; a teacher's
+// entries take eight lanes each, two at a time.
+template <typename T, int kRows, bool TEACHER>
+__global__ void __launch_bounds__(kFinishThreads, TEACHER ? 3 : 5)
+finish_rows_kernel(FinishArgs a) {
   chain_enter();
   constexpr int G = kFinishThreads / kRows, W = kFinishThreads / 32;
-  constexpr int DOTS = 4;
-  extern __shared__ float s_terms[];   // [kRows][k] terms of the teachers' sums
+  static_assert(kRows <= W, "a warp per row");
+  extern __shared__ float s_terms[];   // TEACHER: [kRows][k] terms of the sums
   __shared__ float s_m[W][kRows], s_s[W][kRows];
-  __shared__ float s_lse[kRows];
-  const int n = *count;
+  __shared__ float s_lse[kRows], s_loss[kRows];
+  const int n = *a.count;
   const int base = blockIdx.x * kRows;
   const int live = max(0, min(kRows, n - base));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rr = threadIdx.x % kRows, grp = threadIdx.x / kRows;
+  const T* packed = static_cast<const T*>(a.packed);
+  const T* weight = static_cast<const T*>(a.weight);
+  float z = 0.f, z_product = 0.f;
+  if (!TEACHER && warp < live) {
+    const int c = base + warp;
+    const T* b[1] = {weight + (long long)a.tgt[c] * a.weight_ld};
+    group_dots<T, 32, 1>(packed + (long long)c * a.packed_ld, b, a.width, &z);
+    z_product = a.zt[c];
+  }
   float m = -1e38f, s = 0.f;
   auto merge = [&](float m2, float s2) {
     const float mm = fmaxf(m, m2);
@@ -839,8 +915,8 @@ finish_rows_kernel(const float2* __restrict__ part, long long part_ld, int n_par
   };
   if (rr < live) {
 #pragma unroll 4
-    for (int t = grp; t < n_part; t += G) {
-      const float2 v = part[(long long)t * part_ld + base + rr];
+    for (int t = grp; t < a.n_part; t += G) {
+      const float2 v = a.part[(long long)t * a.part_ld + base + rr];
       merge(v.x, v.y);
     }
   }
@@ -861,64 +937,62 @@ finish_rows_kernel(const float2* __restrict__ part, long long part_ld, int n_par
     s_lse[threadIdx.x] = m * kLn2 + logf(s);
   }
   __syncthreads();
-  if (!idx) {
+  if (!TEACHER) {
+    if (warp < live && lane == 0) {
+      const int r = a.origin[base + warp];
+      const float lse = s_lse[warp], fixed = lse + log1pf(expf(z_product - lse) * expm1f(z - z_product));
+      a.loss_rows[r] = s_loss[warp] = fixed - z;
+      a.lse_rows[r] = fixed;
+    }
+  } else {
+    const int pairs = (a.k + 1) / 2, sub = lane & 7;
+    for (int t0 = warp * 4; t0 < live * pairs; t0 += W * 4) {   // four pairs of entries per warp
+      const int t = min(t0 + (lane >> 3), live * pairs - 1);
+      const int i = t / pairs, e0 = (t - i * pairs) * 2, c = base + i;
+      const long long at = (long long)a.origin[c] * a.k;
+      const bool two = e0 + 1 < a.k;
+      const int cls[2] = {a.idx[at + e0], two ? a.idx[at + e0 + 1] : -1};
+      const T* b[2] = {weight + (long long)max(cls[0], 0) * a.weight_ld, weight + (long long)max(cls[1], 0) * a.weight_ld};
+      float zs[2];
+      group_dots<T, 8, 2>(packed + (long long)c * a.packed_ld, b, a.width, zs);
+      if (sub < 2 && (sub == 0 || two)) {
+        const int e = e0 + sub;
+        const bool counts = cls[sub] >= 0;
+        const float lp = (sub ? zs[1] : zs[0]) * a.inv_t - s_lse[i], qe = a.q[at + e];
+        s_terms[i * a.k + e] = counts && qe != 0.f ? qe * (logf(qe) - lp) : 0.f;
+        a.diff[at + e] = counts ? expf(lp) - a.cw[at + e] : 0.f;
+      }
+    }
+    __syncthreads();
     for (int i = warp; i < live; i += W) {
-      const int c = base + i;
-      const T* b[1] = {weight + (long long)tgt[c] * weight_ld};
-      float z;
-      warp_dots<T, 1>(packed + (long long)c * packed_ld, b, width, &z);
+      float sum = 0.f;
+      for (int e = lane; e < a.k; e += 32) sum += s_terms[i * a.k + e];
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
       if (lane == 0) {
-        const int r = origin[c];
-        const float fixed = s_lse[i] + log1pf(expf(zt[c] - s_lse[i]) * expm1f(z - zt[c]));
-        loss_rows[r] = fixed - z;
-        lse_rows[r] = fixed;
+        const int r = a.origin[base + i];
+        a.loss_rows[r] = s_loss[i] = sum / (a.inv_t * a.inv_t);
+        a.lse_rows[r] = s_lse[i];
       }
     }
   }
-  const int per_row = idx ? (k + DOTS - 1) / DOTS : 0;
-  for (int t = warp; t < live * per_row; t += W) {
-    const int i = t / per_row, e0 = (t - i * per_row) * DOTS, c = base + i;
-    const long long at = (long long)origin[c] * k;
-    const T* b[DOTS];
-    int cls[DOTS];
-#pragma unroll
-    for (int o = 0; o < DOTS; ++o) {
-      cls[o] = e0 + o < k ? idx[at + e0 + o] : -1;
-      b[o] = weight + (long long)(cls[o] < 0 ? 0 : cls[o]) * weight_ld;
-    }
-    float z[DOTS];
-    warp_dots<T, DOTS>(packed + (long long)c * packed_ld, b, width, z);
-    if (lane < DOTS && e0 + lane < k) {
-      const int e = e0 + lane;
-      const float mine = lane == 0 ? z[0] : lane == 1 ? z[1] : lane == 2 ? z[2] : z[3];
-      const int have = lane == 0 ? cls[0] : lane == 1 ? cls[1] : lane == 2 ? cls[2] : cls[3];
-      const float lp = mine * inv_t - s_lse[i], qe = q[at + e];
-      s_terms[i * k + e] = have >= 0 && qe != 0.f ? qe * (logf(qe) - lp) : 0.f;
-      diff[at + e] = have >= 0 ? expf(lp) - cw[at + e] : 0.f;
-    }
-  }
-  if (idx) __syncthreads();
-  for (int i = warp; idx && i < live; i += W) {
-    float sum = 0.f;
-    for (int e = lane; e < k; e += 32) sum += s_terms[i * k + e];
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) {
-      const int r = origin[base + i];
-      loss_rows[r] = sum / (inv_t * inv_t);
-      lse_rows[r] = s_lse[i];
-    }
-  }  // the block that ends last takes the mean: all rows in one order, in 64 bits
+  // the block that ends last takes the mean: the blocks' sums in one order, in 64 bits
   __shared__ bool s_last;
   __shared__ double s_sum[W];
-  __threadfence();
   __syncthreads();
-  if (threadIdx.x == 0) s_last = atomicAdd(done, 1) == (int)gridDim.x - 1;
+  if (threadIdx.x == 0) {
+    double sum = 0.0;
+    for (int i = 0; i < live; ++i) sum += (double)s_loss[i];
+    a.block_sums[blockIdx.x] = sum;
+    __threadfence();
+    s_last = atomicAdd(a.done, 1) == (int)gridDim.x - 1;
+  }
   __syncthreads();
   if (!s_last) return;
   __threadfence();
   double sum = 0.0;
-  for (int r = threadIdx.x; r < rows; r += kFinishThreads) sum += (double)__ldcg(loss_rows + r);
+#pragma unroll 4
+  for (int b = threadIdx.x; b < (int)gridDim.x; b += kFinishThreads) sum += __ldcg(a.block_sums + b);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   if (lane == 0) s_sum[warp] = sum;
@@ -926,8 +1000,8 @@ finish_rows_kernel(const float2* __restrict__ part, long long part_ld, int n_par
   if (threadIdx.x == 0) {
     for (int w = 1; w < W; ++w) sum += s_sum[w];
     const int div = n > 1 ? n : 1;
-    *mean = (float)(sum / div);
-    *inv_live = 1.0f / (float)div;
+    *a.mean = (float)(sum / div);
+    *a.inv_live = 1.0f / (float)div;
   }
 }
 
@@ -975,8 +1049,8 @@ static int make_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t 
   cuuint32_t box[2] = {(cuuint32_t)BK, box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(map, dtype == LANCET_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-                  const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   LANCET_REQUIRE(r == CUDA_SUCCESS, LANCET_ERR_CUDA, "head product: cuTensorMapEncodeTiled failed with code %d", (int)r);
   return LANCET_OK;
 }
@@ -988,7 +1062,7 @@ template <typename T, int FORM, int EPI, bool CTA2, bool ACC>
 static int launch_form(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut, const Params& p, long long units, bool split, int* workers,
                        cudaStream_t st) {
   auto kernel = head_product_kernel<T, FORM, EPI, CTA2, ACC>;
-  constexpr int SMEM = Cfg<CTA2>::SMEM_BYTES;
+  constexpr int SMEM = Cfg<FORM, EPI, CTA2>::SMEM_BYTES;
   static int set_for[64] = {0};   // per device
   int dev = 0;
   LANCET_CUDA(cudaGetDevice(&dev));
@@ -1042,8 +1116,9 @@ static int launch_product_as(const CUtensorMap& tmA, const CUtensorMap& tmB, con
   if constexpr (EPI == EPI_OUT) {
     if (split) {
       const int most = (int)(units < workers ? units : workers);   // tiles that can have been cut
-      const int rows = m < UNIT ? (m + JOIN_ROWS - 1) / JOIN_ROWS : UNIT / JOIN_ROWS;
-      launch_chained(join_tiles_kernel<T, FORM, CTA2>, dim3(most, rows), dim3(256), 0, st, p, workers);
+      const int per = workers >= JOIN_MANY * units ? 1 : JOIN_ROWS;
+      const int rows = m < UNIT ? m : UNIT;
+      launch_chained(join_tiles_kernel<T, FORM, CTA2>, dim3(most, (rows + per - 1) / per), dim3(256), 0, st, p, workers, per);
       return launch_status("join_tiles_kernel");
     }
   }
@@ -1079,6 +1154,7 @@ struct FwdWs {
   float2* part;
   int32_t* tgt;
   int* done;
+  double* block_sums;
   float* zt;
   float* q;
   float* cw;
@@ -1095,6 +1171,7 @@ static FwdWs fwd_ws(void* ws, int rows, int vocab, int width, int k) {
   w.tgt = c.take<int32_t>(k ? 0 : rows);
   w.zt = c.take<float>(k ? 0 : rows);
   w.done = c.take<int>(1);
+  w.block_sums = c.take<double>(rows);
   w.q = c.take<float>((size_t)rows * k);
   w.cw = c.take<float>((size_t)rows * k);
   w.idx = c.take<int32_t>((size_t)rows * k);
@@ -1185,22 +1262,22 @@ struct FwdArgs {
   int32_t* status;
 };
 
-template <typename T>
+template <typename T, bool TEACHER>
 static int finish_launch(const FwdArgs& a, const FwdWs& w, int n_part, cudaStream_t st) {
-  const T* packed = reinterpret_cast<const T*>(w.packed);
-  const T* weight = static_cast<const T*>(a.weight);
+  const FinishArgs f = {w.part, pad_rows(a.rows), n_part, a.pos + a.rows, w.origin, w.packed, pad_width(a.width), a.weight, a.ldw, a.width,
+                        w.tgt, w.zt, w.idx, w.q, w.cw, a.k, a.inv_t, a.loss_rows, a.lse_rows, a.diff, w.block_sums, w.done, a.mean, a.inv_live};
   auto go = [&](auto kernel, int rows_per_block) {
-    const size_t smem = a.target ? 0 : (size_t)rows_per_block * a.k * sizeof(float);   // at most 16 KB
-    launch_chained(kernel, dim3((a.rows + rows_per_block - 1) / rows_per_block), dim3(kFinishThreads), smem, st,
-                   static_cast<const float2*>(w.part), pad_rows(a.rows), n_part, static_cast<const int32_t*>(a.pos + a.rows),
-                   static_cast<const int32_t*>(w.origin), packed, pad_width(a.width), weight, a.ldw, a.width,
-                   static_cast<const int32_t*>(w.tgt), static_cast<const float*>(w.zt), static_cast<const int32_t*>(a.target ? nullptr : w.idx), static_cast<const float*>(w.q), static_cast<const float*>(w.cw), a.k, a.inv_t,
-                   a.loss_rows, a.lse_rows, a.diff, a.rows, w.done, a.mean, a.inv_live);
+    const size_t smem = TEACHER ? (size_t)rows_per_block * a.k * sizeof(float) : 0;   // at most 16 KB
+    launch_chained(kernel, dim3((a.rows + rows_per_block - 1) / rows_per_block), dim3(kFinishThreads), smem, st, f);
     return launch_status("finish_rows_kernel");
   };
   // 8 rows a block read the partial sums in whole sectors; with few rows, more blocks
-  if (a.rows >= 256) return go(finish_rows_kernel<T, 8>, 8);
-  return go(finish_rows_kernel<T, 1>, 1);
+  if (a.rows >= 512) return go(finish_rows_kernel<T, 8, TEACHER>, 8);
+  return go(finish_rows_kernel<T, 1, TEACHER>, 1);
+}
+template <typename T>
+static int finish_launch(const FwdArgs& a, const FwdWs& w, int n_part, cudaStream_t st) {
+  return a.target ? finish_launch<T, false>(a, w, n_part, st) : finish_launch<T, true>(a, w, n_part, st);
 }
 
 static int linear_fwd(const char* fn, const FwdArgs& a, cudaStream_t st) {
@@ -1296,11 +1373,11 @@ static int linear_bwd_t(const BwdArgs& a, const BwdWs& w, cudaStream_t st) {
   if (int rc = make_map(&dzK, w.dz, padded, w.piece, w.piece, BM, a.dtype)) return rc;
   if (int rc = make_map(&wMN, a.weight, a.vocab, a.width, a.ldw, 64, a.dtype)) return rc;
   if (int rc = make_map(&dzMN, w.dz, padded, w.piece, w.piece, 64, a.dtype)) return rc;
-  if (int rc = make_map(&dzOut, w.dz, padded, w.piece, w.piece, OUT_BOX_ROWS, a.dtype)) return rc;
+  if (int rc = make_map(&dzOut, w.dz, padded, w.piece, w.piece, OUT_ROWS, a.dtype)) return rc;
   const bool boxes = a.dweight && a.width % 8 == 0 && aligned(a.dweight, 16);
   dwOut = dzOut;
   if (boxes)   // rows behind the vocabulary are no part of it
-    if (int rc = make_map(&dwOut, a.dweight, a.vocab, a.width, a.width, OUT_BOX_ROWS, a.dtype)) return rc;
+    if (int rc = make_map(&dwOut, a.dweight, a.vocab, a.width, a.width, OUT_ROWS, a.dtype)) return rc;
   if (int rc = make_map(&hMN, w.packed, padded, a.width, pad_width(a.width), 64, a.dtype)) return rc;
   for (int v0 = 0; v0 < a.vocab; v0 += w.piece) {
     const int classes = a.vocab - v0 < w.piece ? a.vocab - v0 : w.piece;
@@ -1355,6 +1432,19 @@ static int linear_bwd(const char* fn, const BwdArgs& a, cudaStream_t st) {
 
 extern "C" {
 using namespace lancet;
+
+int lancet_copy_rows(const void* src, long long lds, void* dst, long long ldd, int rows, int width, lancet_stream_t stream) {
+  LANCET_REQUIRE(rows >= 0 && width >= 1 && lds >= width && ldd >= width && ldd % 8 == 0, LANCET_ERR_INVALID,
+                 "lancet_copy_rows: bad rows=%d, width=%d or row strides %lld / %lld", rows, width, lds, ldd);
+  if (rows == 0) return LANCET_OK;
+  LANCET_REQUIRE(src && dst, LANCET_ERR_NULL, "lancet_copy_rows: null pointer argument");
+  LANCET_REQUIRE(aligned(src, 2) && aligned(dst, 16), LANCET_ERR_INVALID, "lancet_copy_rows: src must be 2-byte, dst 16-byte aligned");
+  int blocks = (rows + 7) / 8;
+  blocks = blocks > 8 * sm_count() ? 8 * sm_count() : blocks;
+  launch_chained(head::copy_rows_kernel, dim3(blocks), dim3(head::kRowThreads), 0, static_cast<cudaStream_t>(stream),
+                 static_cast<const uint16_t*>(src), lds, static_cast<uint16_t*>(dst), ldd, rows, width);
+  return launch_status("copy_rows_kernel");
+}
 
 size_t lancet_linear_loss_fwd_workspace_bytes(int rows, int vocab, int width, int k) {
   if (rows < 0 || vocab < 1 || width < 1 || k < 0) return 0;

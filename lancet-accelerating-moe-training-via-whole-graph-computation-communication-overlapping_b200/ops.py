@@ -394,10 +394,10 @@ def _head_operands(name, hidden, weight, vocab):
                          % (name, tuple(hidden.shape), tuple(weight.shape)))
     vocab = _classes(name, vocab, classes)
     if ldw % 8 or weight.data_ptr() % 16:
-        ldw = (width + 7) // 8 * 8
-        padded = torch.empty((classes, ldw), dtype=weight.dtype, device=weight.device)
-        padded[:, :width] = weight
-        weight = padded
+        ld = (width + 7) // 8 * 8
+        padded = torch.empty((classes, ld), dtype=weight.dtype, device=weight.device)
+        _launch(_capi.lib().lancet_copy_rows, weight, weight.data_ptr(), ldw, padded.data_ptr(), ld, classes, width)
+        weight, ldw = padded, ld
     return hidden, ldh, weight, ldw, vocab
 
 

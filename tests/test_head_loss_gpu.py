@@ -99,7 +99,8 @@ def _run_ce(h, w, target, vocab, up):
     (33, 1009, 1009, 128, torch.float16, 0.2), (127, 257, 300, 72, torch.bfloat16, 0.5), (128, 256, 256, 64, torch.float16, 0.0),
     (129, 255, 256, 65, torch.bfloat16, 0.1), (257, 2000, 2048, 200, torch.bfloat16, 0.9), (300, 777, 777, 513, torch.float16, 0.3),
     (1024, 4099, 4224, 512, torch.bfloat16, 0.02), (2500, 1000, 1000, 96, torch.bfloat16, 0.5), (40, 1009, 1024, 64, torch.bfloat16, 1.0),
-    (513, 3, 3, 1027, torch.bfloat16, 0.0),
+    (513, 3, 3, 1027, torch.bfloat16, 0.0), (200, 700, 700, 240, torch.float16, 0.1), (700, 300, 333, 392, torch.bfloat16, 0.1),
+    (2200, 520, 520, 371, torch.float16, 0.1), (64, 6000, 6000, 1040, torch.bfloat16, 0.0), (90, 3000, 3000, 257, torch.float16, 0.0),
 ])
 def test_linear_cross_entropy(rows, vocab, pad, width, dt, ignored):
     h, w, g = _operands(rows, pad, width, dt, rows + vocab)

@@ -7,7 +7,8 @@ import torch
 import torch.nn.functional as F
 
 from . import _capi
-from .autograd import DeferredGrads, DeferredLinear, LayerNorm, MoE, softmax_cross_entropy
+from .autograd import (DeferredGrads, DeferredLinear, LayerNorm, MoE, distillation_loss, linear_cross_entropy, linear_distillation_loss,
+                       softmax_cross_entropy)
 from .ops import LansState, gemm_status, lans
 
 
@@ -49,14 +50,21 @@ class Block(torch.nn.Module):
 
 class GPTMoE(torch.nn.Module):
     def __init__(self, vocab, m, nh, nl, seq, batch, ffn_dim, world_experts, k=2, capacity_factor=1.25, n_chunks=4,
-                 device="cuda", fabric=None, group=None, seed=0, act="gelu", pipeline=False):
-        """act: activation of every FFN; the reference's GPT-2 uses ReLU (models/benchmark/pytorch/nlp.py:161-165),
+                 device="cuda", fabric=None, group=None, seed=0, act="gelu", pipeline=False, fused_head=False, distill_weight=0.5,
+                 distill_temperature=1.0):
+        """fused_head: the loss is taken from the head's hidden rows without the logits in memory (`linear_cross_entropy`): at
+        8192 tokens and 50257 classes the head needs 1.0 GB beside its operands instead of 1.65 (and no more at larger batches), the
+        step 2 % more time; the default keeps the logits.
+        distill_weight, distill_temperature: share and temperature of the distillation loss where `forward` gets a teacher.
+        act: activation of every FFN; the reference's GPT-2 uses ReLU (models/benchmark/pytorch/nlp.py:161-165),
         its BERT / ViT GELU (:137-141).  pipeline: the MoE blocks run layer norm, gate projection and residual add
         inside the layer's chunk pipeline, and the dense layers queue their weight gradients (DeferredLinear) so that
         they run under the next MoE layer's returning exchange; the trainer joins the queue before the optimizer."""
         super().__init__()
         linear = DeferredLinear if pipeline else torch.nn.Linear
         self.pipeline = bool(pipeline)
+        self.fused_head = bool(fused_head)
+        self.distill_weight, self.distill_temperature = float(distill_weight), float(distill_temperature)
         torch.manual_seed(seed)
         # the tied output projection is a GEMM with the vocabulary as one extent: an odd size (50257) forces the library
         # onto an unaligned legacy kernel that costs a third of the step, so the table is padded to a multiple of 128
@@ -86,17 +94,36 @@ class GPTMoE(torch.nn.Module):
                 out += [b.ffn.w1, b.ffn.b1, b.ffn.w2, b.ffn.b2]
         return out
 
-    def forward(self, ids):
+    def forward(self, ids, teacher=None):
+        """Next-token loss of ids [batch, seq].  teacher: (top_values, top_indices), each [batch, seq, k], a teacher's top logits at every
+        position (torch.topk); positions without one carry negative indices.  The loss is then
+        (1 - distill_weight) * cross entropy + distill_weight * distillation."""
         x = self.emb(ids) + self.pos(torch.arange(ids.shape[1], device=ids.device))[None]
         with torch.autocast("cuda", dtype=torch.bfloat16):
             for b in self.blocks:
                 x = b(x)
-            logits = F.linear(self.ln(x), self.emb.weight)         # tied output embedding
+            rows = self.ln(x)
+            if not self.fused_head:
+                logits = F.linear(rows, self.emb.weight)         # tied output embedding
         # next-token loss on the padded 16-bit logits themselves: position t is scored against token t+1, the last
         # position of every sequence is ignored, the padded vocabulary columns are never read
         target = torch.full_like(ids, -1)
         target[:, :-1] = ids[:, 1:]
-        return softmax_cross_entropy(logits.view(-1, logits.shape[-1]), target.view(-1), self.vocab)
+        if teacher is not None:
+            values, indices = (t.reshape(-1, t.shape[-1]) for t in teacher)
+        if self.fused_head:
+            rows, weight = rows.to(torch.bfloat16).view(-1, rows.shape[-1]), self.emb.weight.to(torch.bfloat16)
+            loss = linear_cross_entropy(rows, weight, target.view(-1), self.vocab)
+            if teacher is not None:
+                soft = linear_distillation_loss(rows, weight, values, indices, self.distill_temperature, self.vocab)
+        else:
+            logits = logits.view(-1, logits.shape[-1])
+            loss = softmax_cross_entropy(logits, target.view(-1), self.vocab)
+            if teacher is not None:
+                soft = distillation_loss(logits, values, indices, self.distill_temperature, self.vocab)
+        if teacher is None:
+            return loss
+        return (1.0 - self.distill_weight) * loss + self.distill_weight * soft
 
     def close(self):
         for b in self.blocks:
@@ -135,11 +162,12 @@ class LansTrainer:
                 off += n
         self._shared_ids = {id(p): i for i, p in enumerate(self.shared)}
 
-    def step(self, ids):
+    def step(self, ids, teacher=None):
+        """One step on token ids; teacher as in `GPTMoE.forward`."""
         self.step_no += 1
         for p in self.params:
             p.grad = None
-        loss = self.model(ids)
+        loss = self.model(ids) if teacher is None else self.model(ids, teacher)
         loss.backward()
         # weight gradients still queued (dense blocks after the last MoE layer of the backward pass) and those running on
         # the side stream must be complete before they are averaged and applied

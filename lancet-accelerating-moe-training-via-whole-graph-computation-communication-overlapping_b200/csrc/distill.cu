@@ -183,17 +183,20 @@ distill_fwd_kernel(const T* __restrict__ x, long long ld, const void* __restrict
   const int head = row_head(row, V);
   const int nv = (V - head) / N;
   const Share sh = share_of(nv, part, parts);
-  const Vec<T>* rv = reinterpret_cast<const Vec<T>*>(row + head);
+  auto get = [&](int v) {   // each value is read once
+    const uint4 q = __ldcs(reinterpret_cast<const uint4*>(row + head) + v);
+    return *reinterpret_cast<const Vec<T>*>(&q);
+  };
   if (sh.first && (int)threadIdx.x < head) add_one(m, s, Num<T>::to_f(row[threadIdx.x]), c);
   int i = sh.v0 + threadIdx.x;
   for (; i + 3 * kThreads < sh.v1; i += 4 * kThreads) {   // four loads in flight
-    const Vec<T> a = rv[i], b = rv[i + kThreads], d = rv[i + 2 * kThreads], e = rv[i + 3 * kThreads];
+    const Vec<T> a = get(i), b = get(i + kThreads), d = get(i + 2 * kThreads), e = get(i + 3 * kThreads);
     add_vec(m, s, a, c);
     add_vec(m, s, b, c);
     add_vec(m, s, d, c);
     add_vec(m, s, e, c);
   }
-  for (; i < sh.v1; i += kThreads) add_vec(m, s, rv[i], c);
+  for (; i < sh.v1; i += kThreads) add_vec(m, s, get(i), c);
   if (sh.last)
     for (int j = head + nv * N + threadIdx.x; j < V; j += kThreads) add_one(m, s, Num<T>::to_f(row[j]), c);
 #pragma unroll
@@ -302,12 +305,19 @@ distill_bwd_kernel(const T* __restrict__ x, long long ld, const long long* __res
   }
 }
 
-// Blocks per row: one is enough to fill the GPU from four blocks per SM on; a share is at least 16 KB of vectors.
-static int parts_for(int rows, int vocab, int bytes) {
+// Threads of a row's block.  A block has fixed steps at both ends (the teacher's softmax, the joins, a last round of loads that does not fill the
+// block), so smaller blocks with more rows under way read faster; the backward pass, which has no such steps, writes long rows faster
+// from large blocks.  8192 x 50304 bf16, 256 / 128 / 64 threads: forward 143 / 132 / 137 us, backward 268 / 276 / 287; 60000 x 4500: forward
+// 338 / 191 / 163, backward 305 / 212 / 183.
+constexpr int SHORT_ROW_BYTES = 16384, SHORT_THREADS = 64, FWD_THREADS = 128, BWD_THREADS = 256;
+static bool short_rows(int vocab, int bytes) { return (long long)vocab * bytes < SHORT_ROW_BYTES; }
+// Blocks per row: several while all of them are resident at once (2048 threads per SM) and each has 16 KB of the row.
+static int parts_for(int rows, int vocab, int bytes, int threads) {
   int parts = 1;
-  while (parts < 8 && 2ll * parts * rows <= 4 * sm_count() && (long long)vocab * bytes / (2 * parts) >= 16384) parts *= 2;
+  while (parts < 8 && 2ll * parts * rows * threads <= 2048ll * sm_count() && (long long)vocab * bytes / (2 * parts) >= 16384) parts *= 2;
   return parts;
 }
+
 // A chained launch, in clusters of `parts` blocks where the kernel joins its blocks' sums.
 template <typename... KArgs, typename... Args>
 static int launch_rows(void (*kernel)(KArgs...), const char* name, int rows, int parts, int threads, bool cluster, cudaStream_t st,
@@ -329,28 +339,24 @@ static int launch_rows(void (*kernel)(KArgs...), const char* name, int rows, int
   return launch_status(name);
 }
 
-// Rows of less than 8 KB take blocks of 64 threads: four times as many rows are under way, and a row's fixed steps (the teacher's softmax, the
-// joins) overlap (9557 rows of 575 float32: 44 + 34 us with 256 threads, 20 + 18 with 64).
-static bool short_rows(int vocab, int bytes) { return (long long)vocab * bytes < 8192; }
-
 template <typename T>
 static int fwd_t(const void* x, long long ld, const void* values, int vdtype, const long long* indices, int k, float inv_t, int rows, int vocab,
                  float* loss, float* lse, float* weights, int32_t* live_rows, cudaStream_t st) {
-  const int parts = parts_for(rows, vocab, sizeof(T));
   const bool few = short_rows(vocab, sizeof(T));
-  return launch_rows(few ? distill_fwd_kernel<T, 64> : distill_fwd_kernel<T, 256>, "distill_fwd_kernel", rows, parts, few ? 64 : 256, true, st,
-                     static_cast<const T*>(x), ld, values, vdtype, indices, k, inv_t, vocab, parts, loss, lse, weights, live_rows);
+  const int threads = few ? SHORT_THREADS : FWD_THREADS, parts = parts_for(rows, vocab, sizeof(T), threads);
+  return launch_rows(few ? distill_fwd_kernel<T, SHORT_THREADS> : distill_fwd_kernel<T, FWD_THREADS>, "distill_fwd_kernel", rows, parts, threads,
+                     true, st, static_cast<const T*>(x), ld, values, vdtype, indices, k, inv_t, vocab, parts, loss, lse, weights, live_rows);
 }
 
 template <typename T>
 static int bwd_t(const void* x, long long ld, const long long* indices, const float* weights, const int32_t* live_rows, int k, float inv_t,
                  int rows, int vocab, int cols, const float* lse, const float* gout, const float* inv_live, float scale, void* dx,
                  long long ldd, cudaStream_t st) {
-  const int parts = parts_for(rows, vocab, sizeof(T));
   const bool few = short_rows(vocab, sizeof(T));
-  return launch_rows(few ? distill_bwd_kernel<T, 64> : distill_bwd_kernel<T, 256>, "distill_bwd_kernel", rows, parts, few ? 64 : 256, false, st,
-                     static_cast<const T*>(x), ld, indices, weights, live_rows, k, inv_t, vocab, cols, parts, lse, gout, inv_live, scale,
-                     static_cast<T*>(dx), ldd);
+  const int threads = few ? SHORT_THREADS : BWD_THREADS, parts = parts_for(rows, vocab, sizeof(T), threads);
+  return launch_rows(few ? distill_bwd_kernel<T, SHORT_THREADS> : distill_bwd_kernel<T, BWD_THREADS>, "distill_bwd_kernel", rows, parts, threads,
+                     false, st, static_cast<const T*>(x), ld, indices, weights, live_rows, k, inv_t, vocab, cols, parts, lse, gout, inv_live,
+                     scale, static_cast<T*>(dx), ldd);
 }
 
 }  // namespace head

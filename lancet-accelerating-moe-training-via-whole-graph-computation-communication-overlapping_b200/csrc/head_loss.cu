@@ -554,18 +554,25 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           const int cols = min(64, left - (c0 & 64)), rows = min(32, d.m - (tl.mt * BM + quad * 32));
           const unsigned long long mine = reinterpret_cast<unsigned long long>(dst + (c0 & 64));
           const unsigned long long first = __shfl_sync(0xffffffffu, mine, 0);
-#pragma unroll 8
-          for (int r = 0; r < 32; ++r) {
-            unsigned char* to = reinterpret_cast<unsigned char*>(p.row_map ? __shfl_sync(0xffffffffu, mine, r)
-                                                                           : first + (unsigned long long)(2 * r) * p.width);
-            const uint32_t word = *reinterpret_cast<const uint32_t*>(box_unit(r, lane >> 2) + (lane & 3) * 4);
-            const uint32_t next = __shfl_down_sync(0xffffffffu, word, 1);
-            const int odd = (reinterpret_cast<uintptr_t>(to) >> 1) & 1;      // elements before the first 4-byte boundary
-            const uint32_t out = odd ? __funnelshift_r(word, next, 16) : word;
-            const int e = r < rows ? 2 * lane + odd : 64;                    // first of this lane's two elements
-            if (e == 1 && lane == 0) *reinterpret_cast<uint16_t*>(to) = (uint16_t)word;
-            if (e + 1 < cols) *reinterpret_cast<uint32_t*>(to + 2 * e) = out;
-            if (e + 1 == cols) *reinterpret_cast<uint16_t*>(to + 2 * e) = (uint16_t)out;
+#pragma unroll 1
+          for (int r0 = 0; r0 < rows; r0 += 8) {   // eight rows' words first, then their stores
+            uint32_t word[8], next[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) word[j] = *reinterpret_cast<const uint32_t*>(box_unit(r0 + j, lane >> 2) + (lane & 3) * 4);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) next[j] = __shfl_down_sync(0xffffffffu, word[j], 1);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int r = r0 + j;
+              unsigned char* to = reinterpret_cast<unsigned char*>(p.row_map ? __shfl_sync(0xffffffffu, mine, r)
+                                                                             : first + (unsigned long long)(2 * r) * p.width);
+              const int odd = (reinterpret_cast<uintptr_t>(to) >> 1) & 1;      // elements before the first 4-byte boundary
+              const uint32_t out = odd ? __funnelshift_r(word[j], next[j], 16) : word[j];
+              const int e = r < rows ? 2 * lane + odd : OUT_COLS;              // first of this lane's two elements
+              if (e == 1 && lane == 0) *reinterpret_cast<uint16_t*>(to) = (uint16_t)word[j];
+              if (e + 1 < cols) *reinterpret_cast<uint32_t*>(to + 2 * e) = out;
+              if (e + 1 == cols) *reinterpret_cast<uint16_t*>(to + 2 * e) = (uint16_t)out;
+            }
           }
           __syncwarp();
         });
@@ -594,8 +601,8 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 }
 
 // Adds the parts of split tiles in a fixed order and finishes them as the product's epilogue does; a thread takes four columns.  Where tiles have
-// many parts (few rows) a block takes one row and its four groups of threads share the parts, else each group has a row of its own.
-constexpr int JOIN_ROWS = 4, JOIN_MANY = 8;
+// many parts (few rows) a block takes one row and its four groups of threads share the parts, else each group has rows of its own.
+constexpr int JOIN_ROWS = 16, JOIN_MANY = 8;
 struct JoinTile {
   int mu, nt, w0, w1, late;   // unit, column tile; first and last worker with a part; whether the first one's is its second part
 };
@@ -660,8 +667,14 @@ __global__ void __launch_bounds__(256) join_tiles_kernel(Params p, int workers, 
     }
   };
   if (rows_per_block == JOIN_ROWS) {
-    const int i = row0 + grp;
-    if (jt.mu * UNIT + i < d.m) finish(i, sum(i, jt.w0, 1));
+    constexpr int N = JOIN_ROWS / 4;
+    float4 v[N];
+#pragma unroll
+    for (int o = 0; o < N; ++o)
+      if (jt.mu * UNIT + row0 + 4 * o + grp < d.m) v[o] = sum(row0 + 4 * o + grp, jt.w0, 1);
+#pragma unroll
+    for (int o = 0; o < N; ++o)
+      if (jt.mu * UNIT + row0 + 4 * o + grp < d.m) finish(row0 + 4 * o + grp, v[o]);
     return;
   }
   s_part[grp][threadIdx.x & 63] = sum(row0, jt.w0 + grp, 4);

@@ -308,7 +308,7 @@ class _LinearLoss(torch.autograd.Function):
     def backward(ctx, gout):
         h, w, target, state = ctx.saved_tensors
         loss, lse, inv_live, pos, diff = ops._state_ptrs(state, h.shape[0])
-        dh, dw = ops._linear_bwd(ctx.name, h, max(h.stride(0), h.shape[1]), w, max(w.stride(0), w.shape[1]), ctx.classes, ctx.vocab, target,
+        dh, dw = ops._linear_bwd(ctx.name, h, ops._row_stride(h), w, ops._row_stride(w), ctx.classes, ctx.vocab, target,
                                  loss, lse, pos, diff if ctx.k else None, ctx.k, ctx.temperature, gout.data_ptr(), inv_live, 1.0,
                                  ctx.needs_input_grad[1], ctx.needs_input_grad[2])
         return None, dh, dw, None, None, None, None
@@ -327,7 +327,7 @@ class _Distillation(torch.autograd.Function):
     def backward(ctx, gout):
         x, indices, state = ctx.saved_tensors
         _, lse, inv_live, live, weights = ops._state_ptrs(state, x.shape[0])
-        return ops._distill_bwd(x, max(x.stride(0), x.shape[1]), indices, ctx.vocab, weights, live, lse, ctx.temperature, gout.data_ptr(),
+        return ops._distill_bwd(x, ops._row_stride(x), indices, ctx.vocab, weights, live, lse, ctx.temperature, gout.data_ptr(),
                                 inv_live, 1.0), None, None, None, None
 
 

@@ -3,15 +3,21 @@
 //     lse[r]  = log sum_j exp(z[r, j] / T)                         (T = 1 for the cross entropy)
 //     loss[r] = lse[r] - z[r, t_r]          or   T^2 sum_i q_i (log q_i - (z[r, idx_i] / T - lse[r])),   q = softmax(v / T)
 //     dz[r, j] = T (exp(z[r, j] / T - lse[r]) - sum_{i: idx_i = j} q_i) g,     dh = dz W,     dW = dz^T h      (one entry with q = 1 for a target)
-// The forward pass is one product whose epilogue reduces each tile's columns to a running maximum and sum per row.  The backward pass walks
-// the vocabulary in pieces: the same product again with an epilogue that writes exp(z / T - lse) of the piece in 16 bits, a small kernel
-// that puts the differences at the targets in place, and two products from that piece.  2 + 2 + 4 flops per row, class and width element.
+// The forward pass is one product whose epilogue reduces each tile's columns to a maximum and a sum per row, and a kernel that joins them and
+// adds the logits at the targets.  The backward pass walks the vocabulary in pieces of up to 1 GiB of dz: the same product again, with an
+// epilogue that writes exp(z / T - lse) in 16 bits (less 1 at a target; a teacher's k differences are placed by a small kernel), and two
+// products from that piece.  2 + 2 + 4 flops per row, class and width element, against 2 + 4 with the logits kept.
 //
-// Rows without a target (or teacher) take no part: a first kernel packs the live rows together (dense rows), every product works on their number, which stays on the device, and the gradient rows go back through the row list.  So an
-// ignored row may hold anything, NaN included, and costs a copy's time only.
+// Rows without a target (or teacher) take no part: the first kernel of each pass packs the live rows together, every product works on their
+// number, which stays on the device, and the gradient rows go back through the row list.  So an ignored row may hold anything, NaN
+// included, and costs a copy's time only.
 //
-// All products run on one kernel: tcgen05.mma from 128-byte-swizzled tiles staged by TMA, float32 accumulators in TMEM, two of them so that
-// the epilogue of one tile runs under the next tile's products.
+// All products run on one kernel: tcgen05.mma on 256 x 256 tiles of a CTA pair (128 x 256 of one CTA up to 128 rows), operands in
+// 128-byte-swizzled tiles staged by TMA, float32 accumulators in TMEM, two of them so that the epilogue of one tile runs under the next
+// tile's products; results leave through shared memory as TMA boxes.  Bound by the tensor cores from a few hundred rows on: at 8192 x 50257 x
+// 1024 bf16 the four products take 533 (sums), 557 (dz), 559 (dh) and 540 us (dW) alone = 1.51 to 1.58 PFLOP/s, 0.94 to 0.99 of the measured
+// burst of a library product; in a loop the power limit holds the step to 2.65 ms (1.27 PFLOP/s, 0.93 of the sustained figure).  With a few
+// rows the weight's bytes bound it (read three times, its gradient written once), below about 100 us the host does.
 #include "head_loss.cuh"
 #include "tcgen05.cuh"
 
@@ -170,7 +176,7 @@ __device__ __forceinline__ void decode_unit(const Params& p, const Dims& d, int 
   if (FORM == FORM_Z) {
     const long long unit_bytes = (long long)(CTA2 ? 2 * BM : BM) * p.width * 2;
     int band = (int)(BAND_BYTES / unit_bytes);
-    band = band < 2 ? 2 : band;
+    band = min(band < 2 ? 2 : band, d.mu);
     const int b = t / (band * d.nt);
     const int in_band = min(band, d.mu - b * band);
     const int r = t - b * band * d.nt;
@@ -1072,8 +1078,8 @@ static int make_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t 
 static bool paired_for(int m) { return m > BM; }
 
 template <typename T, int FORM, int EPI, bool CTA2, bool ACC>
-static int launch_form(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut, const Params& p, long long units, bool split, int* workers,
-                       cudaStream_t st) {
+static int launch_form(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut, const Params& p, long long units, bool split,
+                       int* workers, cudaStream_t st) {
   auto kernel = head_product_kernel<T, FORM, EPI, CTA2, ACC>;
   constexpr int SMEM = Cfg<FORM, EPI, CTA2>::SMEM_BYTES;
   static int set_for[64] = {0};   // per device
@@ -1111,7 +1117,8 @@ static int launch_form(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUt
 }
 
 template <typename T, int FORM, int EPI, bool CTA2>
-static int launch_product_as(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut, const Params& p, int m, int n, int k, cudaStream_t st) {
+static int launch_product_as(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut, const Params& p, int m, int n, int k,
+                             cudaStream_t st) {
   constexpr int UNIT = CTA2 ? 2 * BM : BM;
   const long long units = ((long long)(m + UNIT - 1) / UNIT) * ((n + BN - 1) / BN);
   LANCET_REQUIRE(units < (1ll << 30), LANCET_ERR_INVALID, "head product: %lld tiles", units);
@@ -1139,7 +1146,8 @@ static int launch_product_as(const CUtensorMap& tmA, const CUtensorMap& tmB, con
 }
 // m, n, k: upper bounds of the product's sizes (the live rows are known on the device only)
 template <typename T, int FORM, int EPI>
-static int launch_product(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut, const Params& p, int m, int n, int k, bool paired, cudaStream_t st) {
+static int launch_product(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut, const Params& p, int m, int n, int k,
+                          bool paired, cudaStream_t st) {
   return paired ? launch_product_as<T, FORM, EPI, true>(tmA, tmB, tmOut, p, m, n, k, st)
                 : launch_product_as<T, FORM, EPI, false>(tmA, tmB, tmOut, p, m, n, k, st);
 }

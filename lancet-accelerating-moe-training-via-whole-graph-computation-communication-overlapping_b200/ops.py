@@ -350,11 +350,14 @@ def _matrix(name, what, t):
         raise ValueError("lancet_b200 ops need CUDA tensors (there is no CPU path)")
     if t.dim() != 2:
         raise ValueError("%s: %s must be a matrix" % (name, what))
-    if t.is_contiguous():
-        return t, t.shape[1]
-    if t.stride(1) != 1 or t.stride(0) < t.shape[1]:
+    if not t.is_contiguous() and (t.stride(1) != 1 or t.stride(0) < t.shape[1]):
         t = t.contiguous()
-    return t, max(t.stride(0), t.shape[1])
+    return t, _row_stride(t)
+
+
+def _row_stride(t):
+    """Row stride of what `_matrix` returned (the stride of an axis of length 1 means nothing)."""
+    return t.shape[1] if t.is_contiguous() else t.stride(0)
 
 
 def _classes(name, vocab, most):

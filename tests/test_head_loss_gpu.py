@@ -101,6 +101,7 @@ def _run_ce(h, w, target, vocab, up):
     (1024, 4099, 4224, 512, torch.bfloat16, 0.02), (2500, 1000, 1000, 96, torch.bfloat16, 0.5), (40, 1009, 1024, 64, torch.bfloat16, 1.0),
     (513, 3, 3, 1027, torch.bfloat16, 0.0), (200, 700, 700, 240, torch.float16, 0.1), (700, 300, 333, 392, torch.bfloat16, 0.1),
     (2200, 520, 520, 371, torch.float16, 0.1), (64, 6000, 6000, 1040, torch.bfloat16, 0.0), (90, 3000, 3000, 257, torch.float16, 0.0),
+    (20, 300, 300, 65, torch.float16, 1.0), (1, 1, 1, 13, torch.bfloat16, 0.0),
 ])
 def test_linear_cross_entropy(rows, vocab, pad, width, dt, ignored):
     h, w, g = _operands(rows, pad, width, dt, rows + vocab)
@@ -305,6 +306,63 @@ def test_leading_axes_autocast_and_frozen_operands():
     first = torch.autograd.grad(loss, (h1, w1), retain_graph=True)
     loss.detach().mul_(2)
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, (h1, w1)), first))
+
+
+def test_matrices_of_one_row():
+    """One class or one row taken out of a wider matrix: the stride of an axis of length 1 means nothing."""
+    g = _gen(71)
+    base = torch.randn((9, 29), device=DEV, generator=g).bfloat16()
+    target = torch.zeros(4, dtype=torch.int64, device=DEV)
+    for h, w, t in ((base[:4, :8], base[8:9, :8], target), (base[8:9, :8], base[:4, :8], target[:1])):
+        got = _run_ce(h, w, t, None, 1.0)
+        want = _run_ce(h.clone(memory_format=torch.contiguous_format).reshape(h.shape), w.contiguous().clone().reshape(w.shape), t, None, 1.0)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    x, v, i = base[8:9, 3:20], torch.randn((1, 2), device=DEV, generator=g), torch.tensor([[1, 4]], device=DEV)
+    assert torch.equal(LB.distill_fwd(x, v, i)[1], LB.distill_fwd(x.contiguous().clone(), v, i)[1])
+    _check_distill(x.clone(), v, i, 17, 1.0, torch.bfloat16)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements of weight, gradient and logits: the last rows against the definition."""
+    rows, classes, width, dt = 2, 140000, 16384, torch.bfloat16
+    g = _gen(81)
+    h = torch.randn((rows, width), device=DEV, generator=g).to(dt).requires_grad_()
+    w = torch.zeros((classes, width), dtype=dt, device=DEV)
+    w[-300:] = (torch.randn((300, width), device=DEV, generator=g) * 0.02).to(dt)      # the others have logits of 0
+    w.requires_grad_()
+    target = torch.tensor([classes - 1, classes - 5], device=DEV)
+    loss = LB.linear_cross_entropy(h, w, target)
+    dh, dw = torch.autograd.grad(loss, (h, w))
+    z = h.detach().double() @ w.detach()[-300:].double().t()
+    lse = torch.log(torch.exp(z).sum(dim=1) + (classes - 300))
+    dz = torch.exp(z - lse[:, None])
+    dz[0, -1] -= 1
+    dz[1, -5] -= 1
+    dz /= rows
+    ez = width * 2.0 ** -23 * float((h.detach().double().abs() @ w.detach()[-300:].double().abs().t()).max())
+    assert abs(float(loss.detach()) - float((lse - z[torch.arange(2), target - (classes - 300)]).mean())) <= 2 * ez + 2.0 ** -20 * 20
+    ep = 2 * ez + 2.0 ** -20 * (1 + float(z.abs().max()))
+    err = (U[dt] + ep) * dz.abs() + ep / rows
+    want = dz.t() @ h.detach().double()
+    assert bool(((dw[-300:].double() - want).abs() <= err.t() @ h.detach().double().abs() + U[dt] * want.abs() + 1e-37).all())
+    # dh: the 139700 zero rows add nothing
+    want = dz @ w.detach()[-300:].double()
+    tol = (err + classes * 2.0 ** -23 * dz.abs()) @ w.detach()[-300:].double().abs() + U[dt] * want.abs() + 1e-37
+    assert bool(((dh.double() - want).abs() <= tol).all())
+    del w, dw, dh
+    rows, classes = 43000, 50304
+    x = torch.zeros((rows, classes), dtype=dt, device=DEV)
+    x[-2:] = (torch.randn((2, classes), device=DEV, generator=g) * 3).to(dt)
+    idx = torch.full((rows, 1), -1, device=DEV)
+    idx[-2:] = torch.tensor([[50000], [7]], device=DEV)
+    values = torch.zeros((rows, 1), device=DEV)
+    loss_rows, lse, mean, inv_live, live, weights = LB.distill_fwd(x, values, idx)
+    dx = LB.distill_bwd(x, idx, weights, live, lse, inv_live=inv_live)
+    loss, lse64, dz = _soft(x[-2:].double(), idx[-2:], torch.ones((2, 1), dtype=torch.float64, device=DEV), 1.0)
+    ep = 2.0 ** -20 * (2 + 2 * 20) + (classes / 256 + 16) * 2.0 ** -23
+    assert bool(((loss_rows[-2:].double() - loss).abs() <= ep + 2.0 ** -20 * 20).all()) and float(inv_live) == 0.5
+    assert bool(((dx[-2:].double() - dz / 2).abs() <= (U[dt] + ep) * dz.abs() + ep * (dz < 0) + 1e-37).all())
+    assert not bool(dx[:-2].any())
 
 
 def test_differences_of_the_loss():

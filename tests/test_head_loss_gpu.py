@@ -308,6 +308,27 @@ def test_leading_axes_autocast_and_frozen_operands():
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, (h1, w1)), first))
 
 
+def test_capped_grids_and_plain_launches():
+    """The process-wide knobs of the grouped GEMM hold for the head's products too: fewer workers cut the reductions differently, plain
+    launches give the same bits."""
+    L = LB._capi.lib()
+    for rows, vocab, width in ((300, 3000, 300), (40, 5000, 192)):
+        h, w, g = _operands(rows, vocab, width, torch.bfloat16, rows)
+        target = torch.randint(0, vocab, (rows,), device=DEV, generator=g)
+        live = torch.ones(rows, dtype=torch.bool, device=DEV)
+        want = _run_ce(h, w, target, vocab, 1.0)
+        try:
+            assert L.lancet_set_chained_launch(0) == 0
+            assert all(torch.equal(a, b) for a, b in zip(_run_ce(h, w, target, vocab, 1.0), want))
+            for ctas in (1, 3, 10, 147):
+                assert L.lancet_set_cta_limits(0, ctas) == 0
+                _check_linear(h, w, target[:, None], torch.ones((rows, 1), dtype=torch.float64, device=DEV), live, 1.0, vocab, 1.0,
+                              _run_ce(h, w, target, vocab, 1.0), torch.bfloat16)
+        finally:
+            L.lancet_set_chained_launch(1)
+            L.lancet_set_cta_limits(0, 0)
+
+
 def test_matrices_of_one_row():
     """One class or one row taken out of a wider matrix: the stride of an axis of length 1 means nothing."""
     g = _gen(71)

@@ -1437,14 +1437,16 @@ static int linear_bwd(const char* fn, const BwdArgs& a, cudaStream_t st) {
   LANCET_REQUIRE(a.weight_rows >= a.vocab, LANCET_ERR_INVALID, "%s: %d weight rows for %d classes", fn, a.weight_rows, a.vocab);
   LANCET_REQUIRE(a.rows == 0 || (a.lse_rows && a.pos), LANCET_ERR_NULL, "%s: null pointer argument", fn);
   LANCET_REQUIRE(aligned(a.dhidden, 2) && aligned(a.dweight, 2), LANCET_ERR_INVALID, "%s: outputs are not aligned to their type", fn);
+  const bool work = a.rows > 0 && (a.dhidden || a.dweight);
+  const BwdWs w = bwd_ws(a.ws, a.rows, a.vocab, a.width);
+  if (work)
+    LANCET_REQUIRE(a.ws && aligned(a.ws, 256) && a.ws_bytes >= w.bytes, LANCET_ERR_INVALID,
+                   "%s: workspace missing, not aligned to 256 bytes or smaller than %zu bytes", fn, w.bytes);
   uint16_t* dw = static_cast<uint16_t*>(a.dweight);
   const int first = a.rows == 0 ? 0 : a.vocab;   // rows behind the vocabulary have no gradient
   if (dw && first < a.weight_rows)
     LANCET_CUDA(cudaMemsetAsync(dw + (size_t)first * a.width, 0, (size_t)(a.weight_rows - first) * a.width * 2, st));
-  if (a.rows == 0 || (!a.dhidden && !a.dweight)) return LANCET_OK;
-  const BwdWs w = bwd_ws(a.ws, a.rows, a.vocab, a.width);
-  LANCET_REQUIRE(a.ws && aligned(a.ws, 256) && a.ws_bytes >= w.bytes, LANCET_ERR_INVALID,
-                 "%s: workspace missing, not aligned to 256 bytes or smaller than %zu bytes", fn, w.bytes);
+  if (!work) return LANCET_OK;
   return a.dtype == LANCET_BF16 ? linear_bwd_t<__nv_bfloat16>(a, w, st) : linear_bwd_t<__half>(a, w, st);
 }
 

@@ -216,6 +216,7 @@ distill_fwd_kernel(const T* __restrict__ x, long long ld, const void* __restrict
       s_part[0] = M;
       s_part[1] = S;
     }
+    __syncwarp();
     cluster_barrier();
     if (part == 0 && warp == 0)
       for (int p = 1; p < parts; ++p) merge(M, S, cluster_load(&s_part[0], p), cluster_load(&s_part[1], p), c);

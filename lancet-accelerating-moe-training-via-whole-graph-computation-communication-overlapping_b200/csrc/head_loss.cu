@@ -438,6 +438,7 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           const int owner = __ffs(hits) - 1, col = __shfl_sync(0xffffffffu, want, owner);
           const uint32_t z = tmem_ld1(taddr + col);
           if (lane == owner) p.zt[row] = __uint_as_float(z);
+          __syncwarp();
           hits &= hits - 1;
         }
         float m = -1e30f, s = 0.f;   // maximum of z and sum of 2^((z - m) c)

@@ -4,7 +4,8 @@
 //     loss[r]   = T^2 sum_i q_i (log q_i - (z[r, idx_i] / T - lse[r])),      lse[r] = log sum_j exp(z[r, j] / T)
 //     dz[r, j]  = T (exp(z[r, j] / T - lse[r]) - sum_{i: idx_i = j} q_i) * g     (0 in rows without a teacher and in padded columns)
 // The teacher's tail is not modelled: its top entries are renormalised.  Both passes are bound by HBM: one read of the logits forward, one
-// read and one write backward; q is kept (k numbers per row), the logits' log-probabilities are not.
+// read and one write backward (8192 x 50304 bf16: 129 us = 6.4 TB/s and 263 us = 6.3 TB/s, of 6.5 for a copy); q is kept (k numbers per row),
+// the logits' log-probabilities are not.
 #include "head_loss.cuh"
 #include "tcgen05.cuh"
 
@@ -13,9 +14,10 @@
 namespace lancet {
 namespace head {
 
+constexpr int kMeanThreads = 1024;
 __global__ void __launch_bounds__(kMeanThreads)
-mean_kernel(const float* __restrict__ loss_rows, const int32_t* __restrict__ live_rows, const int32_t* __restrict__ count, int rows,
-            float* __restrict__ mean, float* __restrict__ inv_live) {
+mean_kernel(const float* __restrict__ loss_rows, const int32_t* __restrict__ live_rows, int rows, float* __restrict__ mean,
+            float* __restrict__ inv_live) {
   chain_enter();
   __shared__ double s_sum[kMeanThreads / 32];
   __shared__ int s_live[kMeanThreads / 32];
@@ -23,7 +25,7 @@ mean_kernel(const float* __restrict__ loss_rows, const int32_t* __restrict__ liv
   int live = 0;
   for (int r = threadIdx.x; r < rows; r += kMeanThreads) {
     sum += (double)loss_rows[r];
-    if (live_rows) live += live_rows[r];
+    live += live_rows[r];
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) {
@@ -42,15 +44,14 @@ mean_kernel(const float* __restrict__ loss_rows, const int32_t* __restrict__ liv
       total += s_sum[w];
       n += s_live[w];
     }
-    if (count) n = *count;
     n = n > 1 ? n : 1;
     *mean = (float)(total / n);
     *inv_live = 1.0f / (float)n;
   }
 }
 
-int launch_mean(const float* loss_rows, const int32_t* live_rows, const int32_t* count, int rows, float* mean, float* inv_live, cudaStream_t st) {
-  launch_chained(mean_kernel, dim3(1), dim3(kMeanThreads), 0, st, loss_rows, live_rows, count, rows, mean, inv_live);
+int launch_mean(const float* loss_rows, const int32_t* live_rows, int rows, float* mean, float* inv_live, cudaStream_t st) {
+  launch_chained(mean_kernel, dim3(1), dim3(kMeanThreads), 0, st, loss_rows, live_rows, rows, mean, inv_live);
   return launch_status("mean_kernel");
 }
 
@@ -381,7 +382,7 @@ int lancet_distill_fwd(const void* logits, long long ld, const void* top_values,
     if (int rc = LANCET_DISPATCH_DTYPE(dtype, head::fwd_t, logits, ld, top_values, values_dtype, top_indices, k, 1.0f / temperature, rows,
                                        vocab, loss_rows, lse_rows, class_weights, live_rows, st))
       return rc;
-  return head::launch_mean(loss_rows, live_rows, nullptr, rows, mean, inv_live, st);
+  return head::launch_mean(loss_rows, live_rows, rows, mean, inv_live, st);
 }
 
 int lancet_distill_bwd(const void* logits, long long ld, const long long* top_indices, const float* class_weights, const int32_t* live_rows,

@@ -1303,7 +1303,7 @@ static int finish_launch(const FwdArgs& a, const FwdWs& w, int n_part, cudaStrea
 }
 
 static int linear_fwd(const char* fn, const FwdArgs& a, cudaStream_t st) {
-  if (a.rows == 0) return launch_mean(nullptr, nullptr, nullptr, 0, a.mean, a.inv_live, st);
+  if (a.rows == 0) return launch_mean(nullptr, nullptr, 0, a.mean, a.inv_live, st);
   const FwdWs w = fwd_ws(a.ws, a.rows, a.vocab, a.width, a.target ? 0 : a.k);
   LANCET_REQUIRE(a.ws && aligned(a.ws, 256) && a.ws_bytes >= w.bytes, LANCET_ERR_INVALID,
                  "%s: workspace missing, not aligned to 256 bytes or smaller than %zu bytes", fn, w.bytes);

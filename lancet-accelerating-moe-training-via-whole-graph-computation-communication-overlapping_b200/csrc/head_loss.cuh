@@ -59,12 +59,9 @@ __device__ __forceinline__ float class_weight(const float* q, const int* idx, in
   return s;
 }
 
-// mean = sum of the row losses / max(live rows, 1), inv_live = 1 / max(live rows, 1).  One block, fixed order, 64-bit sums.
-// The live rows are counted from per-row flags, or given as one number.
-constexpr int kMeanThreads = 1024;
-__global__ void mean_kernel(const float* __restrict__ loss_rows, const int32_t* __restrict__ live_rows, const int32_t* __restrict__ count,
-                            int rows, float* __restrict__ mean, float* __restrict__ inv_live);
-int launch_mean(const float* loss_rows, const int32_t* live_rows, const int32_t* count, int rows, float* mean, float* inv_live, cudaStream_t st);
+// mean = sum of the row losses / max(live rows, 1), inv_live = 1 / max(live rows, 1), the live rows counted from per-row flags.  One block,
+// fixed order, 64-bit sums.
+int launch_mean(const float* loss_rows, const int32_t* live_rows, int rows, float* mean, float* inv_live, cudaStream_t st);
 
 }  // namespace head
 }  // namespace lancet

@@ -248,6 +248,9 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  // Earlier kernels' results are read from here on.  TMEM is taken after this wait: a CTA that held it while it waited could keep it from a
+  // kernel that it waits for.
+  chain_enter();
   if (warp == 1) {
     if (CTA2) {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS)
@@ -264,7 +267,6 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   if (CTA2) cluster_sync_all();   // the peer's barriers exist before anything signals them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  chain_enter();                  // the set-up above overlaps the previous kernel's end; its results are read from here on
   const Dims d = dims_of<FORM, CTA2>(p);
   Walk walk(d.mu * d.nt, d.kb, worker, n_workers, EPI == EPI_OUT);
 

@@ -67,7 +67,7 @@ struct Params {
   // EPI_LSE: per (column half tile, row) maximum and sum in the base-2 domain
   float2* part;
   long long part_ld;
-  const int32_t* tgt;     // target of every packed row, or null; its logit goes to zt
+  const int32_t* tgt;     // target (or the teacher's first class) of every packed row; EPI_LSE: its logit goes to zt; EPI_PROB: or null
   float* zt;
   // EPI_PROB: 2^(z c - lse2[row] + shift) of the piece to tmOut, at the rows' targets (tgt) tdiff[row] instead
   const float* lse2;
@@ -393,7 +393,7 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
       }
       if (EPI == EPI_OUT && row_live) out_row = p.row_map ? p.row_map[row] : (long long)p.class0 + row;
-      if (EPI == EPI_LSE && p.tgt && row_live) want = p.tgt[row] - col_first;
+      if (EPI == EPI_LSE && row_live) want = p.tgt[row] - col_first;
       ok = mbar_wait(bar_tfull + 8 * buf, (tphase >> buf) & 1, abort_flag, p.status, 14);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -754,7 +754,7 @@ __device__ __forceinline__ bool row_is_live(const long long* target, const int32
 // counts the live rows before it.  What the buffer holds behind them reaches only results that no one keeps.
 __global__ void __launch_bounds__(kRowThreads)
 pack_rows_kernel(const uint16_t* __restrict__ hidden, long long ld, const long long* __restrict__ target, const int32_t* __restrict__ flags,
-                 int rows, int vocab, int width, uint16_t* __restrict__ packed, int packed_ld, int32_t* __restrict__ origin,
+                 const int32_t* __restrict__ top, int rows, int vocab, int width, uint16_t* __restrict__ packed, int packed_ld, int32_t* __restrict__ origin,
                  int32_t* __restrict__ tgt, int32_t* __restrict__ pos, float* __restrict__ loss_rows, float* __restrict__ lse_rows,
                  int* __restrict__ done) {
   chain_enter();
@@ -786,7 +786,7 @@ pack_rows_kernel(const uint16_t* __restrict__ hidden, long long ld, const long l
       pos[r] = live ? at : -1;
       if (live) {
         origin[at] = r;
-        if (target) tgt[at] = (int)target[r];
+        tgt[at] = target ? (int)target[r] : top[r];
       } else {
         loss_rows[r] = 0.f;
         lse_rows[r] = 0.f;
@@ -888,7 +888,7 @@ struct FinishArgs {
   const void* weight;
   long long weight_ld;
   int width;
-  const int32_t* tgt;      // targets and their logits from the product, by packed row
+  const int32_t* tgt;      // targets (or the teachers' likeliest classes) and their logits from the product, by packed row
   const float* zt;
   const int32_t* idx;      // teachers: classes (-1: none), q, class weights, [rows][k]
   const float* q;
@@ -903,9 +903,9 @@ struct FinishArgs {
 
 // A block finishes kRows packed rows: joins the partial maxima and sums of its rows' column half tiles (in a fixed order), and computes the
 // logits at the rows' targets, or at the entries of their teachers, as float32 dot products.  The tensor cores cut the sums of products short
-// (measured: up to 1e-5 low at a logit of 12), which the loss would show where a target holds most of the probability: its share of the
-// row's sum is replaced by the dot product's.  A target's dot product takes a warp and is under way before the sums are joined; a teacher's
-// entries take eight lanes each, two at a time.
+// (measured: up to 1e-5 low at a logit of 12), which the loss would show where a target (or a teacher's likeliest class) holds most of the
+// probability: its share of the row's sum is replaced by the dot product's.  That dot product takes a warp and is under way before the sums
+// are joined; a teacher's entries take eight lanes each, two at a time.
 template <typename T, int kRows, bool TEACHER>
 __global__ void __launch_bounds__(kFinishThreads, TEACHER ? 3 : 5)
 finish_rows_kernel(FinishArgs a) {
@@ -923,7 +923,7 @@ finish_rows_kernel(FinishArgs a) {
   const T* packed = static_cast<const T*>(a.packed);
   const T* weight = static_cast<const T*>(a.weight);
   float z = 0.f, z_product = 0.f;
-  if (!TEACHER && warp < live) {
+  if (warp < live) {
     const int c = base + warp;
     const T* b[1] = {weight + (long long)a.tgt[c] * a.weight_ld};
     group_dots<T, 32, 1>(packed + (long long)c * a.packed_ld, b, a.width, &z);
@@ -959,14 +959,18 @@ finish_rows_kernel(FinishArgs a) {
     s_lse[threadIdx.x] = m * kLn2 + logf(s);
   }
   __syncthreads();
+  if (warp < live && lane == 0) {   // warp w has the dot product of row w
+    const float lse = s_lse[warp];
+    s_lse[warp] = lse + log1pf(expf(z_product * a.inv_t - lse) * expm1f((z - z_product) * a.inv_t));
+  }
   if (!TEACHER) {
     if (warp < live && lane == 0) {
       const int r = a.origin[base + warp];
-      const float lse = s_lse[warp], fixed = lse + log1pf(expf(z_product - lse) * expm1f(z - z_product));
-      a.loss_rows[r] = s_loss[warp] = fixed - z;
-      a.lse_rows[r] = fixed;
+      a.loss_rows[r] = s_loss[warp] = s_lse[warp] - z;
+      a.lse_rows[r] = s_lse[warp];
     }
   } else {
+    __syncthreads();
     const int pairs = (a.k + 1) / 2, sub = lane & 7;
     for (int t0 = warp * 4; t0 < live * pairs; t0 += W * 4) {   // four pairs of entries per warp
       const int t = min(t0 + (lane >> 3), live * pairs - 1);
@@ -1027,11 +1031,12 @@ finish_rows_kernel(FinishArgs a) {
   }
 }
 
-// Teacher distributions of all rows, a warp each: q, class weights, indices as int32 (-1: does not count), live flags.
+// Teacher distributions of all rows, a warp each: q, class weights, indices as int32 (-1: does not count), the class of the largest q, live
+// flags.
 constexpr int kTeacherWarps = 4;
 __global__ void __launch_bounds__(32 * kTeacherWarps)
 teacher_kernel(const void* __restrict__ values, int vdtype, const long long* __restrict__ indices, int rows, int k, float inv_t, int vocab,
-               float* __restrict__ q, float* __restrict__ cw, int32_t* __restrict__ idx, int32_t* __restrict__ live) {
+               float* __restrict__ q, float* __restrict__ cw, int32_t* __restrict__ idx, int32_t* __restrict__ top, int32_t* __restrict__ live) {
   chain_enter();
   __shared__ float s_q[kTeacherWarps][kMaxTop];
   __shared__ int s_idx[kTeacherWarps][kMaxTop];
@@ -1039,7 +1044,26 @@ teacher_kernel(const void* __restrict__ values, int vdtype, const long long* __r
   const long long r = (long long)blockIdx.x * kTeacherWarps + warp;
   if (r >= rows) return;
   const bool alive = teacher_row(values, vdtype, indices, r, k, inv_t, vocab, s_q[warp], s_idx[warp]);
-  if (lane == 0) live[r] = alive;
+  float best = -1.f;   // largest q and its class; rows with NaN keep class 0
+  int cls = 0;
+  for (int i = lane; i < k; i += 32)
+    if (s_idx[warp][i] >= 0 && s_q[warp][i] > best) {
+      best = s_q[warp][i];
+      cls = s_idx[warp][i];
+    }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    const float b2 = __shfl_xor_sync(0xffffffffu, best, d);
+    const int c2 = __shfl_xor_sync(0xffffffffu, cls, d);
+    if (b2 > best || (b2 == best && c2 < cls)) {
+      best = b2;
+      cls = c2;
+    }
+  }
+  if (lane == 0) {
+    live[r] = alive;
+    top[r] = cls;
+  }
   for (int i = lane; i < k; i += 32) {
     q[r * k + i] = s_q[warp][i];
     cw[r * k + i] = class_weight(s_q[warp], s_idx[warp], k, i);
@@ -1183,6 +1207,7 @@ struct FwdWs {
   float* q;
   float* cw;
   int32_t* idx;
+  int32_t* top;
   int32_t* live;
   size_t bytes;
 };
@@ -1192,13 +1217,14 @@ static FwdWs fwd_ws(void* ws, int rows, int vocab, int width, int k) {
   w.packed = c.take<uint16_t>((size_t)pad_rows(rows) * pad_width(width));
   w.origin = c.take<int32_t>(rows);
   w.part = c.take<float2>((size_t)2 * ((vocab + BN - 1) / BN) * pad_rows(rows));
-  w.tgt = c.take<int32_t>(k ? 0 : rows);
-  w.zt = c.take<float>(k ? 0 : rows);
+  w.tgt = c.take<int32_t>(rows);
+  w.zt = c.take<float>(rows);
   w.done = c.take<int>(1);
   w.block_sums = c.take<double>(rows);
   w.q = c.take<float>((size_t)rows * k);
   w.cw = c.take<float>((size_t)rows * k);
   w.idx = c.take<int32_t>((size_t)rows * k);
+  w.top = c.take<int32_t>(k ? rows : 0);
   w.live = c.take<int32_t>(k ? rows : 0);
   w.bytes = c.used + 256;
   return w;
@@ -1311,13 +1337,13 @@ static int linear_fwd(const char* fn, const FwdArgs& a, cudaStream_t st) {
                  "%s: workspace missing, not aligned to 256 bytes or smaller than %zu bytes", fn, w.bytes);
   if (!a.target) {
     launch_chained(teacher_kernel, dim3((a.rows + kTeacherWarps - 1) / kTeacherWarps), dim3(32 * kTeacherWarps), 0, st, a.values, a.vdtype,
-                   a.indices, a.rows, a.k, a.inv_t, a.vocab, w.q, w.cw, w.idx, w.live);
+                   a.indices, a.rows, a.k, a.inv_t, a.vocab, w.q, w.cw, w.idx, w.top, w.live);
     if (int rc = launch_status("teacher_kernel")) return rc;
   }
   int blocks = (a.rows + 7) / 8;
   blocks = blocks > 4 * 148 ? 4 * 148 : blocks;
   launch_chained(pack_rows_kernel, dim3(blocks), dim3(kRowThreads), 0, st, static_cast<const uint16_t*>(a.hidden), a.ldh, a.target,
-                 static_cast<const int32_t*>(a.target ? nullptr : w.live), a.rows, a.vocab, a.width, w.packed, pad_width(a.width), w.origin,
+                 static_cast<const int32_t*>(a.target ? nullptr : w.live), static_cast<const int32_t*>(w.top), a.rows, a.vocab, a.width, w.packed, pad_width(a.width), w.origin,
                  w.tgt, a.pos, a.loss_rows, a.lse_rows, w.done);
   if (int rc = launch_status("pack_rows_kernel")) return rc;
   const bool paired = paired_for(a.rows);
@@ -1332,7 +1358,7 @@ static int linear_fwd(const char* fn, const FwdArgs& a, cudaStream_t st) {
   p.c = a.inv_t * kLog2e;
   p.part = w.part;
   p.part_ld = pad_rows(a.rows);
-  p.tgt = a.target ? w.tgt : nullptr;
+  p.tgt = w.tgt;
   p.zt = w.zt;
   int rc = a.dtype == LANCET_BF16 ? launch_product<__nv_bfloat16, FORM_Z, EPI_LSE>(tmA, tmB, tmA, p, a.rows, a.vocab, a.width, paired, st)
                                   : launch_product<__half, FORM_Z, EPI_LSE>(tmA, tmB, tmA, p, a.rows, a.vocab, a.width, paired, st);

@@ -107,11 +107,12 @@ __device__ __forceinline__ Dims dims_of(const Params& p) {
 // A reduction over classes or rows is long where the tiles are few.  The workers first take whole tiles in turn as long as each gets one;
 // what is left (`rem` tiles) is cut along the reduction into equal contiguous ranges, a range per worker, so that all of them end together.
 // A range spans two tiles at most; parts of a tile go to float32 slots (2 per worker) and are added in order by join_tiles_kernel.
-// Cutting pays when the idle share of the last turn costs more than the join ((workers - rem) / workers x kb blocks of 512 clocks against
-// about 8000 clocks) and is more than a quarter of all turns: below that the GPU, which runs these products at its power limit, clocks higher
-// while some SMs idle, and the parts' traffic costs more than the turn (8192 rows x 1024, 128 tiles on 74 pairs: 2.67 ms for the
-// step with whole tiles, 2.77 cut).
-constexpr int SPLIT_MIN_KB = 16;
+// Cutting pays when the idle share of the last turn costs more than the parts' way through memory and the join: (workers - rem) / workers x kb
+// blocks of 512 clocks against about 16000 clocks (captured passes, whole tiles / cut: 1 x 50257 x 1024 372 / 121 us, 9000 x 512 x 384 95 / 68,
+// 300 x 3000 x 768 60 / 58; nearest to the limit 3000 x 2000 x 512 74 / 80); and when it is more than a quarter of all turns: below that the
+// GPU, which runs long products at its power limit, clocks higher while some SMs idle (8192 x 50257 x 1024, 128 tiles on 74 pairs: 2.67 /
+// 2.77 ms in a loop).
+constexpr int SPLIT_MIN_KB = 32;
 constexpr int SPLIT_MIN_PART = 4;
 struct Split {
   int full, rem, parts, kb;   // whole tiles, tiles that are cut, ranges they are cut into, blocks of a tile
@@ -610,7 +611,8 @@ head_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 }
 
 // Adds the parts of split tiles in a fixed order and finishes them as the product's epilogue does; a thread takes four columns.  Where tiles have
-// many parts (few rows) a block takes one row and its four groups of threads share the parts, else each group has rows of its own.
+// many parts (few rows) a block takes one row and its four groups of threads share the parts, else each group has rows of its own (captured
+// passes, one row / 16 rows a block: 64 x 50257 x 512 78 / 137 us, 1000 x 6112 x 2080 161 / 140).
 constexpr int JOIN_ROWS = 16, JOIN_MANY = 8;
 struct JoinTile {
   int mu, nt, w0, w1, late;   // unit, column tile; first and last worker with a part; whether the first one's is its second part
@@ -1101,7 +1103,8 @@ static int make_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t 
   return LANCET_OK;
 }
 
-// The paired form halves the bytes of B through shared memory per product; up to 128 rows its second tile would be empty.
+// The paired form halves the bytes of B through shared memory per product; up to 128 rows its second tile would be empty (captured passes at
+// 50257 x 1024, one CTA / pairs: 100 rows 129 / 130 us, 200 rows 171 / 143, 511 rows 267 / 218; 4096 x 32000 x 2048 1.67 / 1.47 ms).
 static bool paired_for(int m) { return m > BM; }
 
 template <typename T, int FORM, int EPI, bool CTA2, bool ACC>
@@ -1321,8 +1324,9 @@ static int finish_launch(const FwdArgs& a, const FwdWs& w, int n_part, cudaStrea
     launch_chained(kernel, dim3((a.rows + rows_per_block - 1) / rows_per_block), dim3(kFinishThreads), smem, st, f);
     return launch_status("finish_rows_kernel");
   };
-  // 8 rows a block read the partial sums in whole sectors; with few rows, more blocks
-  if (a.rows >= 512) return go(finish_rows_kernel<T, 8, TEACHER>, 8);
+  // 8 rows a block read the partial sums in whole sectors; with few rows, more blocks (scoring at 32000 x 256, 1 / 8 rows a block: 512 rows
+  // 23 / 25 us, 1024 rows 33 / 31; with 16 teacher entries 33 / 32 and 45 / 39)
+  if (a.rows > 512) return go(finish_rows_kernel<T, 8, TEACHER>, 8);
   return go(finish_rows_kernel<T, 1, TEACHER>, 1);
 }
 template <typename T>

@@ -346,7 +346,9 @@ def linear_cross_entropy(hidden, weight, target, vocab=None):
     `softmax_cross_entropy(F.linear(hidden, weight), target, vocab)` without the [rows, classes] logits and their gradient in memory.
     hidden [..., width] and weight [classes, width] bfloat16 or float16 of one type (inside an autocast region: cast to its type), target
     [...] int64 (negative or >= vocab = ignored), weight rows from `vocab` on are padding.  The sums are float32; the gradient of the logits
-    passes between the products in the operands' type, as it does between a loss and F.linear."""
+    passes between the products in the operands' type, as it does between a loss and F.linear.
+    Before `backward()` is captured into a CUDA graph, drop losses of the same leaves from outside the capture: torch keeps the leaves'
+    accumulation on the stream of the graph that lives, and work on that stream ends the capture."""
     hidden, weight = _head_inputs(hidden, weight)
     return _LinearLoss.apply("linear_cross_entropy", hidden, weight, vocab, target.reshape(-1), None, 1.0)
 

@@ -484,7 +484,8 @@ int lancet_linear_distill_bwd(const void* hidden, long long ldh, const void* wei
 /* The distillation loss on given logits [rows][ld] (float32, float16 or bfloat16; columns from vocab on are padding and never read), the
  * soft-target counterpart of lancet_softmax_xent_*; teacher, ignored rows, mean and inv_live as above.  class_weights [rows][k] float32 (the
  * teacher's probability of each entry's class) and live_rows [rows] int32 are kept for the backward call, which writes the gradient in the
- * logits' type: zero in padded columns and ignored rows. */
+ * logits' type: zero in padded columns and ignored rows.  live_rows[r] is 0 in ignored rows, in the others the bits of a float32 that is never
+ * +0: log-sum-exp less lse_rows[r], so that logits far from zero keep their differences (from |lse_rows[r]| = 2^24 on: less max z / T instead). */
 int lancet_distill_fwd(const void* logits, long long ld, const void* top_values, int values_dtype, const long long* top_indices, int k,
                        float temperature, int rows, int vocab, int dtype, float* loss_rows, float* lse_rows, float* class_weights,
                        int32_t* live_rows, float* mean, float* inv_live, lancet_stream_t stream);

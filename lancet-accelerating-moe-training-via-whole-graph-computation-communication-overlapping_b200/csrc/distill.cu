@@ -4,8 +4,14 @@
 //     loss[r]   = T^2 sum_i q_i (log q_i - (z[r, idx_i] / T - lse[r])),      lse[r] = log sum_j exp(z[r, j] / T)
 //     dz[r, j]  = T (exp(z[r, j] / T - lse[r]) - sum_{i: idx_i = j} q_i) * g     (0 in rows without a teacher and in padded columns)
 // The teacher's tail is not modelled: its top entries are renormalised.  Both passes are bound by HBM: one read of the logits forward, one
-// read and one write backward (8192 x 50304 bf16: 129 us = 6.4 TB/s and 263 us = 6.3 TB/s, of 6.5 for a copy); q is kept (k numbers per row),
+// read and one write backward (8192 x 50304 bf16: 129 us = 6.4 TB/s and 267 us = 6.2 TB/s, of 6.5 for a copy); q is kept (k numbers per row),
 // the logits' log-probabilities are not.
+//
+// lse = M / T + log S (M the row's largest logit, S the sum of exp((z - M) / T)) loses log S where M / T is large: at 1e4 a tenth of a percent of
+// every probability, and all of it in a row of nothing but the type's lowest value.  So it is kept as two floats, lse[r] rounded and what that
+// rounding left out: live_rows[r] is 0 in rows without a teacher and the bits of that rest in the others (-0 for none).  The backward pass takes
+// differences from a logit near T lse and adds what that one is off, in both floats.  From |lse| = 2^24 on M / T alone fills both (or is beyond
+// float32): there the rest is log S, and the backward pass finds M again.
 #include "head_loss.cuh"
 #include "tcgen05.cuh"
 
@@ -13,6 +19,8 @@
 
 namespace lancet {
 namespace head {
+
+constexpr float kLseTwoFloats = 0x1p24f;   // below it the two floats hold log-sum-exp to 2^-24 of 1 + log S
 
 constexpr int kMeanThreads = 1024;
 __global__ void __launch_bounds__(kMeanThreads)
@@ -25,7 +33,7 @@ mean_kernel(const float* __restrict__ loss_rows, const int32_t* __restrict__ liv
   int live = 0;
   for (int r = threadIdx.x; r < rows; r += kMeanThreads) {
     sum += (double)loss_rows[r];
-    live += live_rows[r];
+    live += live_rows[r] != 0;
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) {
@@ -122,6 +130,12 @@ __device__ __forceinline__ void merge(float& m, float& s, float m2, float s2, fl
   s = s * ex2f((m - mm) * c) + s2 * ex2f((m2 - mm) * c);
   m = mm;
 }
+
+// Threads of a row's block.  A block has fixed steps at both ends (the teacher's softmax, the joins, a last round of loads that does not fill the
+// block), so smaller blocks with more rows under way read faster; the backward pass, which has no such steps, writes long rows faster
+// from large blocks.  8192 x 50304 bf16, 256 / 128 / 64 threads: forward 143 / 132 / 137 us, backward 268 / 276 / 287; 60000 x 4500: forward
+// 338 / 191 / 163, backward 305 / 212 / 183.
+constexpr int SHORT_ROW_BYTES = 16384, SHORT_THREADS = 64, FWD_THREADS = 128, BWD_THREADS = 256;
 
 // A row is read by one block, or with few rows by the blocks of a cluster: contiguous shares of its 16-byte vectors, the maxima and sums
 // joined through the cluster's shared memory in rank order.
@@ -224,22 +238,41 @@ distill_fwd_kernel(const T* __restrict__ x, long long ld, const void* __restrict
     cluster_barrier();   // no block leaves while its sums are read
   }
   if (part == 0 && warp == 0) {
-    const float l = M * inv_t + logf(S);
+    const float log_s = logf(S);
+    const float l = fmaf(M, inv_t, log_s);
+    const float rest = fabsf(l) >= kLseTwoFloats ? log_s : fmaf(M, inv_t, -l) + log_s;
     float sum = 0.f;
     for (int e = lane; e < k; e += 32)
-      if (s_q[e] != 0.f) sum += s_q[e] * (logf(s_q[e]) - (Num<T>::to_f(row[s_idx[e]]) * inv_t - l));
+      if (s_q[e] != 0.f) sum += s_q[e] * (logf(s_q[e]) - ((Num<T>::to_f(row[s_idx[e]]) - M) * inv_t - log_s));
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if (lane == 0) {
       lse[r] = l;
       loss[r] = sum / (inv_t * inv_t);
-      live_rows[r] = 1;
+      live_rows[r] = rest == 0.f ? (int32_t)0x80000000 : __float_as_int(rest);
     }
   }
 }
 
+// Largest value of a row, in all threads of its block.  A call, so that the rows that need it cost the others no registers.
 template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads)
+__device__ __noinline__ float block_max(const T* row, int V) {
+  __shared__ float s_m[kThreads / 32];
+  float m = -INFINITY;
+#pragma unroll 1
+  for (int j = threadIdx.x; j < V; j += kThreads) m = fmaxf(m, Num<T>::to_f(row[j]));
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  if ((threadIdx.x & 31) == 0) s_m[threadIdx.x >> 5] = m;
+  __syncthreads();
+  for (int w = 0; w < kThreads / 32; ++w) m = fmaxf(m, s_m[w]);
+  return m;
+}
+
+// 32 registers a thread: whole SMs of threads.  With the 42 that the compiler takes unbounded (6 blocks of 256 per SM) 8192 x 50304 bf16 ran 259 us
+// for 267, but 500 x 50257 20.0 for 16.8 and 60000 x 4500 187 for 177.
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, kThreads == BWD_THREADS ? 8 : 28)
 distill_bwd_kernel(const T* __restrict__ x, long long ld, const long long* __restrict__ indices, const float* __restrict__ weights,
                    const int32_t* __restrict__ live_rows, int k, float inv_t, int V, int cols, int parts, const float* __restrict__ lse,
                    const float* __restrict__ gout, const float* __restrict__ inv_live, float scale, T* __restrict__ dx, long long ldd) {
@@ -249,9 +282,16 @@ distill_bwd_kernel(const T* __restrict__ x, long long ld, const long long* __res
   const long long r = blockIdx.x / parts;
   const T* row = x + r * ld;
   T* drow = dx + r * ldd;
-  const bool live = live_rows[r] != 0;
+  const int rest = live_rows[r];
+  const bool live = rest != 0;
   const float g = scale * (gout ? *gout : 1.f) * (inv_live ? *inv_live : 1.f) / inv_t;
-  const float c = inv_t * kLog2e, l = lse[r] / inv_t;   // differences of raw values, as in the forward pass
+  const float c = inv_t * kLog2e, l = lse[r];
+  float base = l / inv_t, off = __int_as_float(rest) - fmaf(base, inv_t, -l);   // log-sum-exp = base / T + off
+  if (live && fabsf(l) >= kLseTwoFloats) {   // the same in all threads
+    base = block_max<T, kThreads>(row, V);
+    off = __int_as_float(rest);
+  }
+  const float part_g = ex2f(-off * kLog2e) * g;   // off goes into the factor of the gradient
   // vectors where both rows meet 16-byte boundaries at the same element; the blocks of a row take contiguous shares of them
   const bool same = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(drow)) & 15) == 0;
   const int head = same ? row_head(row, V) : 0;
@@ -259,14 +299,14 @@ distill_bwd_kernel(const T* __restrict__ x, long long ld, const long long* __res
   const Share sh = share_of(nv, part, parts);
   const Vec<T>* rv = reinterpret_cast<const Vec<T>*>(row + head);
   Vec<T>* dv = reinterpret_cast<Vec<T>*>(drow + head);
-  auto grad = [&](float v) { return Num<T>::from_f(ex2f((v - l) * c) * g); };
-  auto grad_vec = [&](const Vec<T>& a) {
+  auto grad = [&](float v) { return Num<T>::from_f(ex2f((v - base) * c) * part_g); };   // differences of raw values, as in the forward pass
+  auto grad_vec = [&](const Vec<T>& v) {
     Vec<T> o;
-    const f32x2 ll = splat2(-l), cc = splat2(c), gg = splat2(g);
+    const f32x2 bb = splat2(-base), cc = splat2(c), gg = splat2(part_g);
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
       float x, y;
-      unpack2(mul2(add2(pack2(Num<T>::to_f(a.v[j]), Num<T>::to_f(a.v[j + 1])), ll), cc), x, y);
+      unpack2(mul2(add2(pack2(Num<T>::to_f(v.v[j]), Num<T>::to_f(v.v[j + 1])), bb), cc), x, y);
       unpack2(mul2(pack2(ex2f(x), ex2f(y)), gg), x, y);
       o.v[j] = Num<T>::from_f(x);
       o.v[j + 1] = Num<T>::from_f(y);
@@ -303,15 +343,10 @@ distill_bwd_kernel(const T* __restrict__ x, long long ld, const long long* __res
   const int to = same ? (sh.last ? V : head + sh.v1 * N) : single.v1;
   for (int e = threadIdx.x; e < k; e += kThreads) {
     const long long at = indices[r * k + e];
-    if (at >= from && at < to && at < V) drow[at] = Num<T>::from_f((ex2f((Num<T>::to_f(row[at]) - l) * c) - weights[r * k + e]) * g);
+    if (at >= from && at < to && at < V) drow[at] = Num<T>::from_f(ex2f((Num<T>::to_f(row[at]) - base) * c) * part_g - weights[r * k + e] * g);
   }
 }
 
-// Threads of a row's block.  A block has fixed steps at both ends (the teacher's softmax, the joins, a last round of loads that does not fill the
-// block), so smaller blocks with more rows under way read faster; the backward pass, which has no such steps, writes long rows faster
-// from large blocks.  8192 x 50304 bf16, 256 / 128 / 64 threads: forward 143 / 132 / 137 us, backward 268 / 276 / 287; 60000 x 4500: forward
-// 338 / 191 / 163, backward 305 / 212 / 183.
-constexpr int SHORT_ROW_BYTES = 16384, SHORT_THREADS = 64, FWD_THREADS = 128, BWD_THREADS = 256;
 static bool short_rows(int vocab, int bytes) { return (long long)vocab * bytes < SHORT_ROW_BYTES; }
 // Blocks per row: several while there are no more than 4 (forward; 8 backward) blocks per SM and each has 16 KB of the row.  50257 bf16, one /
 // several blocks: 7 rows forward 12.7 / 10.6 us, backward 8.4 / 6.3; 500 rows forward 18.8 / 21.0 (so one), backward 18.3 / 16.7.

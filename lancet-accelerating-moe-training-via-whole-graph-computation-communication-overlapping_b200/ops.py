@@ -573,7 +573,8 @@ def _distill_bwd(logits, ld, indices, vocab, weights, live, lse, temperature, gr
 
 def distill_fwd(logits, top_values, top_indices, temperature=1.0, vocab=None):
     """The loss of `linear_distill_fwd` on given logits [rows, cols] (float32, float16 or bfloat16; columns from `vocab` on are padding
-    and never read).  Returns (loss_rows, lse_rows, mean, inv_live, live_rows, class_weights); the last two are kept for `distill_bwd`."""
+    and never read).  Returns (loss_rows, lse_rows, mean, inv_live, live_rows, class_weights); the last two are kept for `distill_bwd`.
+    live_rows (int32) is 0 in ignored rows and nowhere else; its other values hold what the rounding of lse_rows left out."""
     mean, state, logits, indices, _ = _distill_fwd(logits, top_values, top_indices, temperature, vocab)
     rows = logits.shape[0]
     loss, lse, inv_live, live, weights = _state_parts(state, rows, indices.shape[1])

@@ -293,7 +293,7 @@ def softmax_cross_entropy(logits, target, vocab=None):
 
 class _LinearLoss(torch.autograd.Function):
     """The linear losses: a target per row (k = 0), or a teacher's values and indices.  What the forward pass leaves for the backward one is
-    a float and a whole-number tensor; operands are saved as the kernels read them and not checked again."""
+    a float and a whole-number tensor; operands are saved as the kernels read them, and only their strides are looked at again."""
 
     @staticmethod
     def forward(ctx, name, hidden, weight, vocab, target, teacher, temperature):
@@ -308,8 +308,8 @@ class _LinearLoss(torch.autograd.Function):
     def backward(ctx, gout):
         h, w, target, state, pos = ctx.saved_tensors
         loss, lse, inv_live, diff = ops._state_ptrs(state, h.shape[0])
-        dh, dw = ops._linear_bwd(ctx.name, h, ops._row_stride(h), w, ops._row_stride(w), ctx.classes, ctx.vocab, target,
-                                 loss, lse, pos.data_ptr(), diff if ctx.k else None, ctx.k, ctx.temperature, gout.data_ptr(), inv_live, 1.0,
+        dh, dw = ops._linear_bwd(ctx.name, *ops._unpacked(ctx.name, h, w), ctx.classes, ctx.vocab, target.contiguous(), loss, lse,
+                                 pos.data_ptr(), diff if ctx.k else None, ctx.k, ctx.temperature, gout.data_ptr(), inv_live, 1.0,
                                  ctx.needs_input_grad[1], ctx.needs_input_grad[2])
         return None, dh, dw, None, None, None, None
 
@@ -326,8 +326,9 @@ class _Distillation(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gout):
         x, indices, state, live = ctx.saved_tensors
+        x, ld = ops._matrix("distillation_loss", "logits", x)
         _, lse, inv_live, weights = ops._state_ptrs(state, x.shape[0])
-        return ops._distill_bwd(x, ops._row_stride(x), indices, ctx.vocab, weights, live.data_ptr(), lse, ctx.temperature, gout.data_ptr(),
+        return ops._distill_bwd(x, ld, indices.contiguous(), ctx.vocab, weights, live.data_ptr(), lse, ctx.temperature, gout.data_ptr(),
                                 inv_live, 1.0), None, None, None, None
 
 

@@ -396,12 +396,25 @@ def _head_operands(name, hidden, weight, vocab):
         raise ValueError("%s: hidden [rows, width] and weight [classes, width] on one device do not match: %s, %s"
                          % (name, tuple(hidden.shape), tuple(weight.shape)))
     vocab = _classes(name, vocab, classes)
-    if ldw % 8 or weight.data_ptr() % 16:
-        ld = (width + 7) // 8 * 8
-        padded = torch.empty((classes, ld), dtype=weight.dtype, device=weight.device)
-        _launch(_capi.lib().lancet_copy_rows, weight, weight.data_ptr(), ldw, padded.data_ptr(), ld, classes, width)
-        weight, ldw = padded, ld
+    weight, ldw = _aligned_rows(weight, ldw, width)
     return hidden, ldh, weight, ldw, vocab
+
+
+def _aligned_rows(weight, ldw, width):
+    """The weight and its row stride with rows on 16-byte boundaries: itself, or a copy with a padded row stride."""
+    if ldw % 8 == 0 and weight.data_ptr() % 16 == 0:
+        return weight, ldw
+    classes, ld = weight.shape[0], (width + 7) // 8 * 8
+    padded = torch.empty((classes, ld), dtype=weight.dtype, device=weight.device)
+    _launch(_capi.lib().lancet_copy_rows, weight, weight.data_ptr(), ldw, padded.data_ptr(), ld, classes, width)
+    return padded, ld
+
+
+def _unpacked(name, hidden, weight):
+    """Saved operands, with their row strides, as a saved-tensor hook may have given them back: the same values with other strides."""
+    hidden, ldh = _matrix(name, "hidden", hidden)
+    weight, ldw = _matrix(name, "weight", weight)
+    return (hidden, ldh, *_aligned_rows(weight, ldw, hidden.shape[1]))
 
 
 def _head_status(device):

@@ -1,4 +1,5 @@
-"""What the head's losses save for their backward passes, taken through saved-tensor hooks: floating-point tensors stored in fewer bits."""
+"""What the head's losses save for their backward passes, taken through saved-tensor hooks: floating-point tensors stored in fewer bits, and
+tensors moved to the host and back (other strides)."""
 import pytest
 import torch
 
@@ -43,3 +44,13 @@ def test_saved_floats_in_fewer_bits():
             assert bool(torch.isfinite(a).all())
             # |lse| is at most log 300 + 8 here; every gradient is a sum of probability differences times operands
             assert float((a.double() - b.double()).norm()) <= (2.0 ** -7 * 14 + 2.0 ** -7) * float(b.double().norm())
+
+
+def test_saved_tensors_moved_to_the_host():
+    """What comes back has the same values and no gaps between its rows."""
+    args = _inputs()
+    want = [torch.autograd.grad(loss, leaves) for loss, leaves in _losses(*args)]
+    with torch.autograd.graph.save_on_cpu():
+        losses = _losses(*args)
+    for (loss, leaves), ref in zip(losses, want):
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, leaves), ref))

@@ -417,14 +417,6 @@ def _unpacked(name, hidden, weight):
     return (hidden, ldh, *_aligned_rows(weight, ldw, hidden.shape[1]))
 
 
-def _head_status(device):
-    """The status word of the bounded waits (`gemm_status`).  A word first made under stream capture would be filled by the replay
-    only: such a call gets one of its own."""
-    if device not in _gemm_status and torch.cuda.is_current_stream_capturing():
-        return torch.zeros(1, dtype=torch.int32, device=device)
-    return gemm_status(device)
-
-
 def _grad_scalar(name, t, like):
     if t is None:
         return None
@@ -477,7 +469,7 @@ def _linear_fwd(name, hidden, weight, vocab, target=None, teacher=None, temperat
     nws = L.lancet_linear_loss_fwd_workspace_bytes(rows, vocab, width, k)
     ws = torch.empty(nws, dtype=torch.uint8, device=hidden.device)
     operands = (hidden.data_ptr(), ldh, w.data_ptr(), ldw)
-    end = (mean.data_ptr(), inv_live, ws.data_ptr(), nws, _head_status(hidden.device).data_ptr())
+    end = (mean.data_ptr(), inv_live, ws.data_ptr(), nws, gemm_status(hidden.device).data_ptr())
     if teacher is None:
         _launch(L.lancet_linear_xent_fwd, hidden, *operands, target.data_ptr(), rows, vocab, width, _DT[hidden.dtype], loss, lse,
                 pos.data_ptr(), *end)
@@ -497,7 +489,7 @@ def _linear_bwd(name, hidden, ldh, w, ldw, classes, vocab, target, loss, lse, po
     nws = L.lancet_linear_loss_bwd_workspace_bytes(rows, vocab, width)
     ws = torch.empty(nws, dtype=torch.uint8, device=hidden.device)
     end = (rows, vocab, classes, width, _DT[hidden.dtype], grad_out, inv_live, scale, None if dh is None else dh.data_ptr(),
-           None if dw is None else dw.data_ptr(), ws.data_ptr(), nws, _head_status(hidden.device).data_ptr())
+           None if dw is None else dw.data_ptr(), ws.data_ptr(), nws, gemm_status(hidden.device).data_ptr())
     if diff is None:
         _launch(L.lancet_linear_xent_bwd, hidden, hidden.data_ptr(), ldh, w.data_ptr(), ldw, target.data_ptr(), loss, lse, pos, *end)
     else:
@@ -615,14 +607,45 @@ def distill_bwd(logits, top_indices, class_weights, live_rows, lse_rows, tempera
 
 ACT = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3}
 _gemm_status = {}
+_filling = {}   # words first made under capture, with the event behind their first fill
 
 
 def gemm_status(device):
-    """Device status word of the grouped GEMM (non-zero after a bounded wait gave up)."""
+    """Device status word of the bounded waits of the grouped GEMM and the head's products (non-zero after one gave up): one per device."""
+    st = _gemm_status.get(device)
+    return st if st is not None else _status_word(device)
+
+
+def _status_word(device):
+    """The word where it is not made yet, is still being filled, or is asked for under another name of the device.  A word first made under
+    stream capture comes from the graph's memory, where it is kept for good, and is filled at once on a stream that is not captured: the graph
+    neither takes it over nor fills it again."""
+    name, device = device, torch.device(device)
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
     st = _gemm_status.get(device)
     if st is None:
-        st = torch.zeros(1, dtype=torch.int32, device=device)
-        _gemm_status[device] = st
+        with torch.cuda.device(device):
+            if not torch.cuda.is_current_stream_capturing():
+                st, filled = _filling.pop(device, (None, None))
+                if st is None:
+                    st = torch.zeros(1, dtype=torch.int32, device=device)
+                else:
+                    torch.cuda.current_stream().wait_event(filled)
+                _gemm_status[device] = st
+            elif device in _filling:
+                return _filling[device][0]
+            else:
+                st = torch.empty(1, dtype=torch.int32, device=device)
+                for side in (torch.cuda.Stream() for _ in range(64)):
+                    with torch.cuda.stream(side):
+                        if not torch.cuda.is_current_stream_capturing():
+                            st.zero_()
+                            _filling[device] = st, side.record_event()
+                            return st
+                raise RuntimeError("gemm_status: every stream is being captured; call it once before the capture")
+    if torch.device(name).index is not None:   # without an index: the device that is current at each call
+        _gemm_status[name] = st
     return st
 
 

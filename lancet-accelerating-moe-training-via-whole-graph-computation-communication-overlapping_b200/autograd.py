@@ -357,6 +357,9 @@ def linear_cross_entropy(hidden, weight, target, vocab=None):
 def linear_distillation_loss(hidden, weight, top_values, top_indices, temperature=1.0, vocab=None):
     """`distillation_loss` of the language-model head from its hidden rows, without the logits in memory; hidden and weight as for
     `linear_cross_entropy`, top_values and top_indices [..., k]."""
+    if top_indices.dim() < 1 or top_values.shape[-1:] != top_indices.shape[-1:]:
+        raise ValueError("linear_distillation_loss: top_values %s and top_indices %s must both be [..., k]"
+                         % (tuple(top_values.shape), tuple(top_indices.shape)))
     hidden, weight = _head_inputs(hidden, weight)
     k = top_indices.shape[-1]
     return _LinearLoss.apply("linear_distillation_loss", hidden, weight, vocab, None,

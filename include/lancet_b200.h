@@ -453,7 +453,7 @@ int lancet_softmax_xent_bwd(const void* logits, long long ld, const long long* t
  * target [rows] int64, negative or >= vocab = row ignored.  Teacher: top_values [rows][k] (float32, float16 or bfloat16) and
  * top_indices [rows][k] int64, k <= 512; an index that names no class does not count, a class named twice gets both weights, a row whose
  * counting values are none or all -inf is ignored.  Ignored rows: loss and lse 0, gradient row 0, and their hidden rows are not used (they
- * may hold anything).  0.001 <= temperature <= 1000.
+ * may hold anything).  0.001 <= temperature <= 1000.  At most 2^26 rows and classes, 2^20 width; 2^30 rows and columns where the logits are given.
  * pos [rows + 1] int32: packed index of every row that takes part or -1, then their number; diff [rows][k] float32: student minus teacher
  * probability at the teacher's classes; the backward calls take both.  mean = sum(loss_rows) * inv_live, inv_live = 1 / max(live rows, 1)
  * (float32 scalars on the device).

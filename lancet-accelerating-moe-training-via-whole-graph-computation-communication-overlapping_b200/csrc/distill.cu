@@ -407,7 +407,8 @@ using namespace lancet;
 int lancet_distill_fwd(const void* logits, long long ld, const void* top_values, int values_dtype, const long long* top_indices, int k,
                        float temperature, int rows, int vocab, int dtype, float* loss_rows, float* lse_rows, float* class_weights,
                        int32_t* live_rows, float* mean, float* inv_live, lancet_stream_t stream) {
-  LANCET_REQUIRE(rows >= 0 && vocab >= 1 && ld >= vocab && valid_dtype(dtype) && valid_dtype(values_dtype), LANCET_ERR_INVALID,
+  LANCET_REQUIRE(rows >= 0 && rows <= head::kMostSize && vocab >= 1 && vocab <= head::kMostSize && ld >= vocab && valid_dtype(dtype) &&
+                     valid_dtype(values_dtype), LANCET_ERR_INVALID,
                  "lancet_distill_fwd: bad rows=%d, vocab=%d, row stride %lld or dtype", rows, vocab, ld);
   LANCET_REQUIRE(k >= 1 && k <= head::kMaxTop, LANCET_ERR_INVALID, "lancet_distill_fwd: k=%d top entries (1 to %d)", k, head::kMaxTop);
   LANCET_REQUIRE(temperature >= 1e-3f && temperature <= 1e3f, LANCET_ERR_INVALID, "lancet_distill_fwd: temperature %g outside [0.001, 1000]",
@@ -425,7 +426,8 @@ int lancet_distill_fwd(const void* logits, long long ld, const void* top_values,
 int lancet_distill_bwd(const void* logits, long long ld, const long long* top_indices, const float* class_weights, const int32_t* live_rows,
                        int k, float temperature, int rows, int vocab, int cols, int dtype, const float* lse_rows, const float* grad_out,
                        const float* inv_live, float scale, void* dlogits, long long ldd, lancet_stream_t stream) {
-  LANCET_REQUIRE(rows >= 0 && vocab >= 1 && cols >= vocab && ld >= vocab && ldd >= cols && valid_dtype(dtype), LANCET_ERR_INVALID,
+  LANCET_REQUIRE(rows >= 0 && rows <= head::kMostSize && vocab >= 1 && cols >= vocab && cols <= head::kMostSize && ld >= vocab && ldd >= cols &&
+                     valid_dtype(dtype), LANCET_ERR_INVALID,
                  "lancet_distill_bwd: bad rows=%d, vocab=%d, cols=%d, row strides %lld / %lld or dtype", rows, vocab, cols, ld, ldd);
   LANCET_REQUIRE(k >= 1 && k <= head::kMaxTop, LANCET_ERR_INVALID, "lancet_distill_bwd: k=%d top entries (1 to %d)", k, head::kMaxTop);
   LANCET_REQUIRE(temperature >= 1e-3f && temperature <= 1e3f, LANCET_ERR_INVALID, "lancet_distill_bwd: temperature %g outside [0.001, 1000]",

@@ -1490,7 +1490,8 @@ extern "C" {
 using namespace lancet;
 
 int lancet_copy_rows(const void* src, long long lds, void* dst, long long ldd, int rows, int width, lancet_stream_t stream) {
-  LANCET_REQUIRE(rows >= 0 && width >= 1 && lds >= width && ldd >= width && ldd % 8 == 0, LANCET_ERR_INVALID,
+  LANCET_REQUIRE(rows >= 0 && rows <= head::kMostSize && width >= 1 && width <= head::kMostSize && lds >= width && ldd >= width && ldd % 8 == 0,
+                 LANCET_ERR_INVALID,
                  "lancet_copy_rows: bad rows=%d, width=%d or row strides %lld / %lld", rows, width, lds, ldd);
   if (rows == 0) return LANCET_OK;
   LANCET_REQUIRE(src && dst, LANCET_ERR_NULL, "lancet_copy_rows: null pointer argument");

@@ -10,6 +10,7 @@ namespace head {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kMostSize = 1 << 30;   // rows or columns: 32-bit counters step past the end by less than as much again
 constexpr int kMaxTop = 512;   // entries of a teacher's row: they are held in shared memory
 
 __device__ __forceinline__ float ex2f(float x) {

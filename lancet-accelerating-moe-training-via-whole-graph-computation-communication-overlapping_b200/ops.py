@@ -350,6 +350,8 @@ def _matrix(name, what, t):
         raise ValueError("lancet_b200 ops need CUDA tensors (there is no CPU path)")
     if t.dim() != 2:
         raise ValueError("%s: %s must be a matrix" % (name, what))
+    if max(t.shape) >> 31:
+        raise ValueError("%s: %s has more rows or columns than 32 bits count: %s" % (name, what, tuple(t.shape)))
     if not t.is_contiguous() and (t.stride(1) != 1 or t.stride(0) < t.shape[1]):
         t = t.contiguous()
     return t, _row_stride(t)
@@ -379,6 +381,8 @@ def _teacher_rows(name, top_values, top_indices, like):
     if top_indices.dim() != 2 or top_values.shape != top_indices.shape or top_indices.shape[0] != like.shape[0] or \
             top_values.device != like.device or top_indices.device != like.device:
         raise ValueError("%s: the teacher's values and indices must be [rows, k] on the operands' device" % name)
+    if top_indices.shape[1] >> 31:
+        raise ValueError("%s: more entries per row than 32 bits count: %s" % (name, tuple(top_indices.shape)))
     if top_indices.dtype != torch.int64 or top_values.dtype not in _DT:
         raise TypeError("%s: top_indices must be int64, the values float32, float16 or bfloat16" % name)
     return top_values.contiguous(), top_indices.contiguous()

@@ -1,4 +1,4 @@
-"""Calls of the head's losses that are refused: teachers whose values and indices do not belong together."""
+"""Calls of the head's losses that are refused: teachers whose values and indices do not belong together, and sizes past 32 bits."""
 import pytest
 import torch
 
@@ -18,3 +18,19 @@ def test_teacher_of_other_shapes():
             LB.linear_distillation_loss(h, w, v, i)
     want = LB.linear_distillation_loss(h, w, values.view(6, 2), idx)
     assert torch.equal(LB.linear_distillation_loss(h.view(2, 3, 16), w, values.view(2, 3, 2), idx), want)     # leading axes as they come
+
+
+def test_sizes_past_32_bits():
+    """More rows, classes or entries than 32 bits count (one element seen many times, so that it takes no memory) are not taken for the few that
+    remain of their number in 32 bits."""
+    one = torch.zeros((1, 1), dtype=torch.bfloat16, device=DEV)
+    t, v, i = torch.zeros(1, dtype=torch.int64, device=DEV), torch.zeros((1, 1), device=DEV), torch.zeros((1, 1), dtype=torch.int64, device=DEV)
+    for n in (2 ** 31, 2 ** 32 + 1):
+        many = one.expand(n, 1)
+        for bad in (lambda: LB.linear_cross_entropy(many, one, t.expand(n)), lambda: LB.linear_cross_entropy(one, many, t),
+                    lambda: LB.linear_distillation_loss(many, one, v.expand(n, 1), i.expand(n, 1)),
+                    lambda: LB.linear_distillation_loss(one, one, v.expand(1, n), i.expand(1, n)),
+                    lambda: LB.distillation_loss(many, v.expand(n, 1), i.expand(n, 1)), lambda: LB.distillation_loss(one.expand(1, n), v, i),
+                    lambda: LB.distillation_loss(one, v.expand(1, n), i.expand(1, n))):
+            with pytest.raises(ValueError):
+                bad()

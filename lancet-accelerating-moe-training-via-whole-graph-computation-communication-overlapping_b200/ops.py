@@ -525,12 +525,12 @@ def linear_distill_fwd(hidden, weight, top_values, top_indices, temperature=1.0,
     return loss, lse, mean, inv_live, pos, diff
 
 
-def _check_saved(name, hidden, lse_rows, pos, *more):
-    rows = hidden.shape[0]
-    _require_cuda(lse_rows, pos, *more)
-    if any(t.device != hidden.device for t in (lse_rows, pos, *more)) or any(t.dtype != torch.float32 for t in (lse_rows, *more)) or \
-            pos.dtype != torch.int32 or lse_rows.shape != (rows,) or pos.shape != (rows + 1,) or any(t.shape[0] != rows for t in more):
-        raise ValueError("%s: the saved tensors must be those of the forward call" % name)
+def _check_saved(name, like, whole, whole_shape, *floats):
+    """An int32 tensor and pairs of a float32 tensor and its shape, contiguous and on the operands' device."""
+    for t, shape in ((whole, whole_shape), *floats):
+        _require_cuda(t)
+        if t.shape != shape or t.dtype != (torch.int32 if t is whole else torch.float32) or t.device != like.device:
+            raise ValueError("%s: the saved tensors must be those of the forward call" % name)
 
 
 def linear_xent_bwd(hidden, weight, target, loss_rows, lse_rows, pos, vocab=None, grad_out=None, inv_live=None, scale=1.0,
@@ -542,7 +542,8 @@ def linear_xent_bwd(hidden, weight, target, loss_rows, lse_rows, pos, vocab=None
     classes = weight.shape[0]
     hidden, ldh, w, ldw, vocab = _head_operands(name, hidden, weight, vocab)
     target = _target_rows(name, target, hidden)
-    _check_saved(name, hidden, lse_rows, pos, loss_rows)
+    rows = hidden.shape[0]
+    _check_saved(name, hidden, pos, (rows + 1,), (lse_rows, (rows,)), (loss_rows, (rows,)))
     return _linear_bwd(name, hidden, ldh, w, ldw, classes, vocab, target, loss_rows.data_ptr(), lse_rows.data_ptr(), pos.data_ptr(), None, 0,
                        1.0, _grad_scalar(name, grad_out, hidden), _grad_scalar(name, inv_live, hidden), float(scale), need_hidden, need_weight)
 
@@ -554,7 +555,8 @@ def linear_distill_bwd(hidden, weight, top_indices, diff, lse_rows, pos, tempera
     classes = weight.shape[0]
     hidden, ldh, w, ldw, vocab = _head_operands(name, hidden, weight, vocab)
     _, top_indices = _teacher_rows(name, diff, top_indices, hidden)
-    _check_saved(name, hidden, lse_rows, pos, diff)
+    rows = hidden.shape[0]
+    _check_saved(name, hidden, pos, (rows + 1,), (lse_rows, (rows,)), (diff, top_indices.shape))
     return _linear_bwd(name, hidden, ldh, w, ldw, classes, vocab, top_indices, None, lse_rows.data_ptr(), pos.data_ptr(), diff.data_ptr(),
                        top_indices.shape[1], float(temperature), _grad_scalar(name, grad_out, hidden), _grad_scalar(name, inv_live, hidden),
                        float(scale), need_hidden, need_weight)
@@ -601,10 +603,8 @@ def distill_bwd(logits, top_indices, class_weights, live_rows, lse_rows, tempera
     _dt(logits)
     vocab = _classes(name, vocab, logits.shape[1])
     _, indices = _teacher_rows(name, class_weights, top_indices, logits)
-    _require_cuda(class_weights, live_rows, lse_rows)
-    if class_weights.dtype != torch.float32 or lse_rows.dtype != torch.float32 or live_rows.dtype != torch.int32 or \
-            lse_rows.shape != logits.shape[:1] or live_rows.shape != logits.shape[:1]:
-        raise ValueError("%s: class_weights, live_rows and lse_rows must be those of the forward call" % name)
+    rows = logits.shape[0]
+    _check_saved(name, logits, live_rows, (rows,), (lse_rows, (rows,)), (class_weights, indices.shape))
     return _distill_bwd(logits, ld, indices, vocab, class_weights.data_ptr(), live_rows.data_ptr(), lse_rows.data_ptr(), float(temperature),
                         _grad_scalar(name, grad_out, logits), _grad_scalar(name, inv_live, logits), float(scale))
 

@@ -1,4 +1,5 @@
-"""Calls of the head's losses that are refused: teachers whose values and indices do not belong together, and sizes past 32 bits."""
+"""Calls of the head's losses that are refused: teachers whose values and indices do not belong together, sizes past 32 bits,
+and saved tensors other than those of the forward call."""
 import pytest
 import torch
 
@@ -34,3 +35,23 @@ def test_sizes_past_32_bits():
                     lambda: LB.distillation_loss(one, v.expand(1, n), i.expand(1, n))):
             with pytest.raises(ValueError):
                 bad()
+
+
+def test_saved_tensors_of_another_shape_or_type():
+    """What the operators' backward forms take back: each tensor in turn replaced by one of another shape, type, stride or place."""
+    rows, classes, width, k = 6, 30, 16, 2
+    h, w = torch.zeros((rows, width), dtype=torch.bfloat16, device=DEV), torch.zeros((classes, width), dtype=torch.bfloat16, device=DEV)
+    t, x = torch.zeros(rows, dtype=torch.int64, device=DEV), torch.zeros((rows, classes), device=DEV)
+    v, i = torch.zeros((rows, k), device=DEV), torch.zeros((rows, k), dtype=torch.int64, device=DEV)
+    loss, lse, _, _, pos = LB.linear_xent_fwd(h, w, t)
+    _, lse2, _, _, pos2, diff = LB.linear_distill_fwd(h, w, v, i)
+    _, lse3, _, _, live, weights = LB.distill_fwd(x, v, i)
+    for call, saved in ((lambda s: LB.linear_xent_bwd(h, w, t, *s), (loss, lse, pos)),
+                        (lambda s: LB.linear_distill_bwd(h, w, i, *s), (diff, lse2, pos2)),
+                        (lambda s: LB.distill_bwd(x, i, *s), (weights, live, lse3))):
+        call(saved)
+        for n, good in enumerate(saved):
+            wide = torch.stack((good, good), dim=-1)
+            for bad in (wide, wide[..., 0], good[:-1], good[0], good.cpu(), good.double(), good.to(torch.int64)):
+                with pytest.raises((ValueError, TypeError)):
+                    call(saved[:n] + (bad,) + saved[n + 1:])

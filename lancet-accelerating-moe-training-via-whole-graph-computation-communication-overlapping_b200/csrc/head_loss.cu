@@ -107,12 +107,16 @@ __device__ __forceinline__ Dims dims_of(const Params& p) {
 // A reduction over classes or rows is long where the tiles are few.  The workers first take whole tiles in turn as long as each gets one;
 // what is left (`rem` tiles) is cut along the reduction into equal contiguous ranges, a range per worker, so that all of them end together.
 // A range spans two tiles at most; parts of a tile go to float32 slots (2 per worker) and are added in order by join_tiles_kernel.
-// Cutting pays when the idle share of the last turn costs more than the parts' way through memory and the join: (workers - rem) / workers x kb
-// blocks of 512 clocks against about 16000 clocks (captured passes, whole tiles / cut: 1 x 50257 x 1024 372 / 121 us, 9000 x 512 x 384 95 / 68,
-// 300 x 3000 x 768 60 / 58; nearest to the limit 3000 x 2000 x 512 74 / 80); and when it is more than a quarter of all turns: below that the
-// GPU, which runs long products at its power limit, clocks higher while some SMs idle (8192 x 50257 x 1024, 128 tiles on 74 pairs: 2.67 /
-// 2.77 ms in a loop).
-constexpr int SPLIT_MIN_KB = 32;
+// Cutting pays when the idle share of the last turn, (workers - rem) / workers x kb blocks of 512 clocks, costs more than the parts' way through
+// memory and their sum: from 32 blocks on for a few tiles, whose parts stay small, and from 56 on for more (the sides meet between 50 and 62
+// blocks).  Captured passes of one gradient, whole tiles / cut, us: few: dW of 2500 rows, 1 tile, 39 blocks 25.9 / 23.0; dh of 300 x 2500 x 768,
+// 6 tiles, 37 blocks 29.2 / 28.4, at 2000 classes, 29 blocks 26.9 / 27.9.  More: dW of 3000 x 2000 x 512, 16 tiles, 37 blocks 35.3 / 41.5, of 5000
+// rows, 62 blocks 49.0 / 48.3; dh of 2264 x 3500 x 256, 9 tiles, 48 blocks 37.6 / 39.2; of 8152 x 6000 x 256, 32 tiles, 53 blocks 82.0 / 79.2; of
+// 100 x 4300 x 7680, 30 tiles, 54 blocks 95.6 / 102.5.  And it pays when that share is more than a
+// quarter of all turns: below that the GPU, which runs long products at its power limit, clocks higher while some SMs idle (8192 x 50257 x 1024,
+// 128 tiles on 74 pairs: 2.67 / 2.77 ms in a loop).
+constexpr int SPLIT_MIN_KB = 32, SPLIT_MIN_KB_MANY = 56;
+constexpr int SPLIT_FEW = 12;   // few: as many workers for each tile
 constexpr int SPLIT_MIN_PART = 4;
 struct Split {
   int full, rem, parts, kb;   // whole tiles, tiles that are cut, ranges they are cut into, blocks of a tile
@@ -123,7 +127,8 @@ __host__ __device__ __forceinline__ Split split_of(int n_tiles, int kb, int work
   Split s = {n_tiles, 0, 1, kb, 0};
   const int rem = n_tiles % workers;
   const long long idle = workers - rem, turns = (n_tiles + workers - 1) / workers;
-  if (rem > 0 && idle * kb > (long long)SPLIT_MIN_KB * workers && 4 * idle > turns * workers) {
+  const long long min_kb = workers >= SPLIT_FEW * rem ? SPLIT_MIN_KB : SPLIT_MIN_KB_MANY;
+  if (rem > 0 && idle * kb > min_kb * workers && 4 * idle > turns * workers) {
     s.full = n_tiles - rem;
     s.rem = rem;
     s.iters = (long long)rem * kb;

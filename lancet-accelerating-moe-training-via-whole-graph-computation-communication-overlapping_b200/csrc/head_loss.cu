@@ -1329,9 +1329,11 @@ static int finish_launch(const FwdArgs& a, const FwdWs& w, int n_part, cudaStrea
     launch_chained(kernel, dim3((a.rows + rows_per_block - 1) / rows_per_block), dim3(kFinishThreads), smem, st, f);
     return launch_status("finish_rows_kernel");
   };
-  // 8 rows a block read the partial sums in whole sectors; with few rows, more blocks (scoring at 32000 x 256, 1 / 8 rows a block: 512 rows
-  // 23 / 25 us, 1024 rows 33 / 31; with 16 teacher entries 33 / 32 and 45 / 39)
-  if (a.rows > 512) return go(finish_rows_kernel<T, 8, TEACHER>, 8);
+  // 8 rows a block read the partial sums in whole sectors; with few rows, or many entries of teachers, more blocks (captured forward passes, 1 / 8
+  // rows a block: targets at 32000 x 256 512 rows 21.5 / 22.3 us, 1024 rows 30.7 / 29.3; teachers at 50257 x 1024 k = 16 640 rows 82 / 88, 1024
+  // rows 108 / 104; k = 64 1536 rows 171 / 194, 2972 rows 322 / 299; k = 256 4096 rows 717 / 844, at 32000 x 256 6000 rows 356 / 337)
+  constexpr int ENTRY_ROWS = 20;
+  if (a.rows > 512 + (TEACHER ? ENTRY_ROWS * a.k : 0)) return go(finish_rows_kernel<T, 8, TEACHER>, 8);
   return go(finish_rows_kernel<T, 1, TEACHER>, 1);
 }
 template <typename T>

@@ -1352,7 +1352,7 @@ static int linear_fwd(const char* fn, const FwdArgs& a, cudaStream_t st) {
     if (int rc = launch_status("teacher_kernel")) return rc;
   }
   int blocks = (a.rows + 7) / 8;
-  blocks = blocks > 4 * 148 ? 4 * 148 : blocks;
+  blocks = blocks > 4 * sm_count() ? 4 * sm_count() : blocks;
   launch_chained(pack_rows_kernel, dim3(blocks), dim3(kRowThreads), 0, st, static_cast<const uint16_t*>(a.hidden), a.ldh, a.target,
                  static_cast<const int32_t*>(a.target ? nullptr : w.live), static_cast<const int32_t*>(w.top), a.rows, a.vocab, a.width, w.packed, pad_width(a.width), w.origin,
                  w.tgt, a.pos, a.loss_rows, a.lse_rows, w.done);
@@ -1408,7 +1408,7 @@ static int linear_bwd_t(const BwdArgs& a, const BwdWs& w, cudaStream_t st) {
   const float shift = a.dtype == LANCET_F16 ? 14.f : 0.f;
   const float unit = a.dtype == LANCET_F16 ? 16384.f : 1.f;
   int blocks = (a.rows + 7) / 8;
-  blocks = blocks > 4 * 148 ? 4 * 148 : (blocks < 8 ? 8 : blocks);   // the zero rows want some warps even for one row
+  blocks = blocks > 4 * sm_count() ? 4 * sm_count() : (blocks < 8 ? 8 : blocks);   // the zero rows want some warps even for one row
   launch_chained(repack_rows_kernel, dim3(blocks), dim3(kRowThreads), 0, st, static_cast<const uint16_t*>(a.hidden), a.ldh, a.pos, a.lse_rows,
                  a.target, a.loss_rows, unit, a.rows, a.width, w.packed, pad_width(a.width), w.origin, w.lse2, w.tgt, w.tdiff,
                  static_cast<uint16_t*>(a.dhidden));

@@ -293,12 +293,12 @@ def softmax_cross_entropy(logits, target, vocab=None):
 
 class _LinearLoss(torch.autograd.Function):
     """The linear losses: a target per row (k = 0), or a teacher's values and indices.  What the forward pass leaves for the backward one is
-    a float and a whole-number tensor; operands are saved as the kernels read them, and only their strides are looked at again."""
+    one buffer; operands are saved as the kernels read them, and only their strides are looked at again."""
 
     @staticmethod
     def forward(ctx, name, hidden, weight, vocab, target, teacher, temperature):
-        mean, state, pos, h, w, target, ctx.vocab = ops._linear_fwd(name, hidden, weight, vocab, target, teacher, temperature)
-        ctx.save_for_backward(h, w, target, state, pos)
+        mean, state, h, w, target, ctx.vocab = ops._linear_fwd(name, hidden, weight, vocab, target, teacher, temperature)
+        ctx.save_for_backward(h, w, target, state)
         ctx.name, ctx.classes, ctx.k = name, weight.shape[0], 0 if teacher is None else target.shape[1]
         ctx.temperature = float(temperature)
         return mean
@@ -306,10 +306,10 @@ class _LinearLoss(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        h, w, target, state, pos = ctx.saved_tensors
-        loss, lse, inv_live, diff = ops._state_ptrs(state, h.shape[0])
-        dh, dw = ops._linear_bwd(ctx.name, *ops._unpacked(ctx.name, h, w), ctx.classes, ctx.vocab, target.contiguous(), loss, lse,
-                                 pos.data_ptr(), diff if ctx.k else None, ctx.k, ctx.temperature, gout.data_ptr(), inv_live, 1.0,
+        h, w, target, state = ctx.saved_tensors
+        loss, lse, inv_live, pos, diff = ops._state_ptrs(state, h.shape[0])
+        dh, dw = ops._linear_bwd(ctx.name, *ops._unpacked(ctx.name, h, w), ctx.classes, ctx.vocab, target, loss, lse,
+                                 pos, diff if ctx.k else None, ctx.k, ctx.temperature, gout.data_ptr(), inv_live, 1.0,
                                  ctx.needs_input_grad[1], ctx.needs_input_grad[2])
         return None, dh, dw, None, None, None, None
 
@@ -317,18 +317,18 @@ class _LinearLoss(torch.autograd.Function):
 class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_values, top_indices, temperature, vocab):
-        mean, state, live, x, indices, ctx.vocab = ops._distill_fwd(logits, top_values, top_indices, temperature, vocab)
-        ctx.save_for_backward(x, indices, state, live)
+        mean, state, x, indices, ctx.vocab = ops._distill_fwd(logits, top_values, top_indices, temperature, vocab)
+        ctx.save_for_backward(x, indices, state)
         ctx.temperature = float(temperature)
         return mean
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        x, indices, state, live = ctx.saved_tensors
-        x, ld = ops._matrix("distillation_loss", "logits", x)
-        _, lse, inv_live, weights = ops._state_ptrs(state, x.shape[0])
-        return ops._distill_bwd(x, ld, indices.contiguous(), ctx.vocab, weights, live.data_ptr(), lse, ctx.temperature, gout.data_ptr(),
+        x, indices, state = ctx.saved_tensors
+        x, ld = (x, x.shape[1]) if x.is_contiguous() else ops._matrix("distillation_loss", "logits", x)
+        _, lse, inv_live, live, weights = ops._state_ptrs(state, x.shape[0])
+        return ops._distill_bwd(x, ld, indices, ctx.vocab, weights, live, lse, ctx.temperature, gout.data_ptr(),
                                 inv_live, 1.0), None, None, None, None
 
 

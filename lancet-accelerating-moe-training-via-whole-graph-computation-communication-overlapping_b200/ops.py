@@ -350,7 +350,7 @@ def _matrix(name, what, t):
         raise ValueError("lancet_b200 ops need CUDA tensors (there is no CPU path)")
     if t.dim() != 2:
         raise ValueError("%s: %s must be a matrix" % (name, what))
-    if max(t.shape) >> 31:
+    if t.numel() >> 31 and max(t.shape) >> 31:
         raise ValueError("%s: %s has more rows or columns than 32 bits count: %s" % (name, what, tuple(t.shape)))
     if not t.is_contiguous() and (t.stride(1) != 1 or t.stride(0) < t.shape[1]):
         t = t.contiguous()
@@ -416,6 +416,8 @@ def _aligned_rows(weight, ldw, width):
 
 def _unpacked(name, hidden, weight):
     """Saved operands, with their row strides, as a saved-tensor hook may have given them back: the same values with other strides."""
+    if hidden.is_contiguous() and weight.is_contiguous() and weight.shape[1] % 8 == 0 and weight.data_ptr() % 16 == 0:
+        return hidden, hidden.shape[1], weight, weight.shape[1]
     hidden, ldh = _matrix(name, "hidden", hidden)
     weight, ldw = _matrix(name, "weight", weight)
     return (hidden, ldh, *_aligned_rows(weight, ldw, hidden.shape[1]))
@@ -440,26 +442,27 @@ def _launch(fn, like, *args):
 
 
 def _state(like, rows, k):
-    """What a forward pass leaves behind: the mean; loss_rows, lse_rows, inv_live and k numbers per row in one float32 allocation; rows + 1
-    int32 (pos, or live_rows and a spare).  Whole numbers have a tensor of their own: a saved-tensor hook may store floats in fewer bits."""
+    """What a forward pass leaves behind, in one allocation: the bits of loss_rows, lse_rows and inv_live, pos (rows + 1; or live_rows and a
+    spare), the bits of k numbers per row; with the mean as a tensor of its own.  An int32 tensor: a saved-tensor hook may store floats in
+    fewer bits, which row numbers do not survive."""
     device = like.device
-    return (torch.empty((), dtype=torch.float32, device=device), torch.empty(rows * (2 + k) + 1, dtype=torch.float32, device=device),
-            torch.empty(rows + 1, dtype=torch.int32, device=device))
+    return (torch.empty((), dtype=torch.float32, device=device), torch.empty(rows * (3 + k) + 2, dtype=torch.int32, device=device))
 
 
 def _state_parts(state, rows, k):
-    """(loss_rows, lse_rows, inv_live, the k numbers per row) as views."""
-    loss, lse, inv_live, more = state.split((rows, rows, 1, rows * k))
-    return loss, lse, inv_live, more.view(rows, k)
+    """(loss_rows, lse_rows, inv_live, pos, the k numbers per row) as views."""
+    floats = state.view(torch.float32)
+    loss, lse, inv_live, _, more = floats.split((rows, rows, 1, rows + 1, rows * k))
+    return loss, lse, inv_live, state[2 * rows + 1:3 * rows + 2], more.view(rows, k)
 
 
 def _state_ptrs(state, rows):
     p = state.data_ptr()
-    return p, p + 4 * rows, p + 8 * rows, p + 8 * rows + 4
+    return p, p + 4 * rows, p + 8 * rows, p + 8 * rows + 4, p + 12 * rows + 8
 
 
 def _linear_fwd(name, hidden, weight, vocab, target=None, teacher=None, temperature=1.0):
-    """Forward pass of the linear losses: (mean, state, row list, operands as the kernels read them)."""
+    """Forward pass of the linear losses: (mean, state, operands as the kernels read them)."""
     hidden, ldh, w, ldw, vocab = _head_operands(name, hidden, weight, vocab)
     rows, width = hidden.shape
     L = _capi.lib()
@@ -468,19 +471,18 @@ def _linear_fwd(name, hidden, weight, vocab, target=None, teacher=None, temperat
     else:
         values, target = _teacher_rows(name, *teacher, hidden)
         k = target.shape[1]
-    mean, state, pos = _state(hidden, rows, k)
-    loss, lse, inv_live, diff = _state_ptrs(state, rows)
+    mean, state = _state(hidden, rows, k)
+    loss, lse, inv_live, pos, diff = _state_ptrs(state, rows)
     nws = L.lancet_linear_loss_fwd_workspace_bytes(rows, vocab, width, k)
     ws = torch.empty(nws, dtype=torch.uint8, device=hidden.device)
     operands = (hidden.data_ptr(), ldh, w.data_ptr(), ldw)
     end = (mean.data_ptr(), inv_live, ws.data_ptr(), nws, gemm_status(hidden.device).data_ptr())
     if teacher is None:
-        _launch(L.lancet_linear_xent_fwd, hidden, *operands, target.data_ptr(), rows, vocab, width, _DT[hidden.dtype], loss, lse,
-                pos.data_ptr(), *end)
+        _launch(L.lancet_linear_xent_fwd, hidden, *operands, target.data_ptr(), rows, vocab, width, _DT[hidden.dtype], loss, lse, pos, *end)
     else:
         _launch(L.lancet_linear_distill_fwd, hidden, *operands, values.data_ptr(), _DT[values.dtype], target.data_ptr(), k, float(temperature),
-                rows, vocab, width, _DT[hidden.dtype], loss, lse, diff, pos.data_ptr(), *end)
-    return mean, state, pos, hidden, w, target, vocab
+                rows, vocab, width, _DT[hidden.dtype], loss, lse, diff, pos, *end)
+    return mean, state, hidden, w, target, vocab
 
 
 def _linear_bwd(name, hidden, ldh, w, ldw, classes, vocab, target, loss, lse, pos, diff, k, temperature, grad_out, inv_live, scale,
@@ -508,8 +510,8 @@ def linear_xent_fwd(hidden, weight, target, vocab=None):
     inv_live, pos): row losses and log-sum-exp (0 in ignored rows), the mean over the other rows, 1 / their number, and the int32 row list
     that `linear_xent_bwd` takes.  The workspace is allocated per call: calls on other streams and captured graphs share nothing.  As with
     the grouped GEMM a wait that ran out is recorded in `gemm_status`."""
-    mean, state, pos, hidden = _linear_fwd("linear_xent_fwd", hidden, weight, vocab, target=target)[:4]
-    loss, lse, inv_live, _ = _state_parts(state, hidden.shape[0], 0)
+    mean, state, hidden = _linear_fwd("linear_xent_fwd", hidden, weight, vocab, target=target)[:3]
+    loss, lse, inv_live, pos, _ = _state_parts(state, hidden.shape[0], 0)
     return loss, lse, mean, inv_live, pos
 
 
@@ -519,9 +521,9 @@ def linear_distill_fwd(hidden, weight, top_values, top_indices, temperature=1.0,
     top_values [rows, k] float32, float16 or bfloat16, top_indices [rows, k] int64, k <= 512; an index that names no class does not
     count (NaN in its value included), a row without counting entries is ignored.  Returns (loss_rows, lse_rows, mean, inv_live, pos, diff)
     as `linear_xent_fwd` does; diff [rows, k] float32 is the student's minus the teacher's probability at the entries."""
-    mean, state, pos, hidden, _, top_indices, _ = _linear_fwd("linear_distill_fwd", hidden, weight, vocab,
-                                                              teacher=(top_values, top_indices), temperature=temperature)
-    loss, lse, inv_live, diff = _state_parts(state, hidden.shape[0], top_indices.shape[1])
+    mean, state, hidden, _, top_indices, _ = _linear_fwd("linear_distill_fwd", hidden, weight, vocab, teacher=(top_values, top_indices),
+                                                         temperature=temperature)
+    loss, lse, inv_live, pos, diff = _state_parts(state, hidden.shape[0], top_indices.shape[1])
     return loss, lse, mean, inv_live, pos, diff
 
 
@@ -569,11 +571,11 @@ def _distill_fwd(logits, top_values, top_indices, temperature, vocab):
     vocab = _classes(name, vocab, logits.shape[1])
     values, indices = _teacher_rows(name, top_values, top_indices, logits)
     rows, k = logits.shape[0], indices.shape[1]
-    mean, state, live = _state(logits, rows, k)
-    loss, lse, inv_live, weights = _state_ptrs(state, rows)
+    mean, state = _state(logits, rows, k)
+    loss, lse, inv_live, live, weights = _state_ptrs(state, rows)
     _launch(_capi.lib().lancet_distill_fwd, logits, logits.data_ptr(), ld, values.data_ptr(), _DT[values.dtype], indices.data_ptr(), k,
-            float(temperature), rows, vocab, dt, loss, lse, weights, live.data_ptr(), mean.data_ptr(), inv_live)
-    return mean, state, live, logits, indices, vocab
+            float(temperature), rows, vocab, dt, loss, lse, weights, live, mean.data_ptr(), inv_live)
+    return mean, state, logits, indices, vocab
 
 
 def _distill_bwd(logits, ld, indices, vocab, weights, live, lse, temperature, grad_out, inv_live, scale):
@@ -588,9 +590,9 @@ def distill_fwd(logits, top_values, top_indices, temperature=1.0, vocab=None):
     """The loss of `linear_distill_fwd` on given logits [rows, cols] (float32, float16 or bfloat16; columns from `vocab` on are padding
     and never read).  Returns (loss_rows, lse_rows, mean, inv_live, live_rows, class_weights); the last two are kept for `distill_bwd`.
     live_rows (int32) is 0 in ignored rows and nowhere else; its other values hold what the rounding of lse_rows left out."""
-    mean, state, live, logits, indices, _ = _distill_fwd(logits, top_values, top_indices, temperature, vocab)
+    mean, state, logits, indices, _ = _distill_fwd(logits, top_values, top_indices, temperature, vocab)
     rows = logits.shape[0]
-    loss, lse, inv_live, weights = _state_parts(state, rows, indices.shape[1])
+    loss, lse, inv_live, live, weights = _state_parts(state, rows, indices.shape[1])
     return loss, lse, mean, inv_live, live[:rows], weights
 
 

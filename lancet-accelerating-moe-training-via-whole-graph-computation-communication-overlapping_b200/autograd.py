@@ -369,7 +369,9 @@ def linear_distillation_loss(hidden, weight, top_values, top_indices, temperatur
 def distillation_loss(logits, top_values, top_indices, temperature=1.0, vocab=None):
     """Mean over rows of T^2 KL(q || softmax(logits / T)), q = softmax(top_values / T) over a teacher's top entries (torch.topk of its logits:
     top_values [rows, k], top_indices [rows, k] int64; an index that names no class does not count, a row without entries is ignored).
-    logits [rows, cols] float32, float16 or bfloat16, columns from `vocab` on are padding.  No gradient goes to the teacher."""
+    logits [rows, cols] float32, float16 or bfloat16, columns from `vocab` on are padding (name them so: with logits[:, :vocab] the rows of
+    the gradient start on other boundaries than the logits', and the backward pass takes up to three times as long).  No gradient goes to
+    the teacher."""
     return _Distillation.apply(logits, top_values.detach(), top_indices, temperature, vocab)
 
 

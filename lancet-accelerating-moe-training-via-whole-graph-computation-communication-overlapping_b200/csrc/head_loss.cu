@@ -1,12 +1,18 @@
 // Losses of the language-model head from its hidden rows, without keeping the logits: cross entropy against target tokens and distillation
-// from a teacher's top logits, forward and backward.  With h [rows][width], W [classes][width] and z = h W^T (never in memory as a whole),
+// from a teacher's top logits, forward and backward.  With h [rows][width], W [classes][width] and z = h W^T (never in memory),
 //     lse[r]  = log sum_j exp(z[r, j] / T)                         (T = 1 for the cross entropy)
 //     loss[r] = lse[r] - z[r, t_r]          or   T^2 sum_i q_i (log q_i - (z[r, idx_i] / T - lse[r])),   q = softmax(v / T)
 //     dz[r, j] = T (exp(z[r, j] / T - lse[r]) - sum_{i: idx_i = j} q_i) g,     dh = dz W,     dW = dz^T h      (one entry with q = 1 for a target)
 // The forward pass is one product whose epilogue reduces each tile's columns to a maximum and a sum per row, and a kernel that joins them and
-// adds the logits at the targets.  The backward pass walks the vocabulary in pieces of up to 1 GiB of dz: the same product again, with an
-// epilogue that writes exp(z / T - lse) in 16 bits (less 1 at a target; a teacher's k differences are placed by a small kernel), and two
-// products from that piece.  2 + 2 + 4 flops per row, class and width element, against 2 + 4 with the logits kept.
+// adds the logits at the targets.  The backward pass walks the vocabulary in pieces of up to 1 GiB of dz (8192 x 50257: all of it in one piece): the
+// same product again, with an epilogue that writes exp(z / T - lse) in 16 bits (less 1 at a target; a teacher's k differences are placed by a
+// small kernel), and two products from that piece.  2 + 2 + 4 flops per row, class and width element, against 2 + 4 with the logits kept.
+//
+// Roundings: dz goes to the tensor cores in the operands' 16 bits, the one rounding beside the results' own, where a loss on 16-bit logits rounds its
+// gradient too; products of a float32 dz would take several 16-bit products or tf32's half rate.  Distance of dh and dW from the definition at
+// 8192 x 50257 x 1024 bf16: 1.9e-3 and 2.0e-3 relative, 1.7e-3 with a float32 dz, 3.0e-3 with 16-bit logits kept.  z is what the tensor cores sum,
+// which they cut short (see finish_rows_kernel), and enters exp2 by one fused multiply-add, so a probability carries some 2^-23 |z| / T.  Log-sum-exp is
+// one float32: its rounding of 2^-24 |lse| is below that.
 //
 // Rows without a target (or teacher) take no part: the first kernel of each pass packs the live rows together, every product works on their
 // number, which stays on the device, and the gradient rows go back through the row list.  So an ignored row may hold anything, NaN
@@ -911,7 +917,8 @@ struct FinishArgs {
 // A block finishes kRows packed rows: joins the partial maxima and sums of its rows' column half tiles (in a fixed order), and computes the
 // logits at the rows' targets, or at the entries of their teachers, as float32 dot products.  The tensor cores cut the sums of products short
 // (measured: up to 1e-5 low at a logit of 12), which the loss would show where a target (or a teacher's likeliest class) holds most of the
-// probability: its share of the row's sum is replaced by the dot product's.  That dot product takes a warp and is under way before the sums
+// probability: its share of the row's sum is replaced by the dot product's.  The other classes keep what was cut: a common offset of 100 in all logits
+// makes the loss 1.4e-4 low at width 1024 (6e-4 at 4096), about what float32 logits scatter by (1.3e-4, 2.8e-4).  That dot product takes a warp and is under way before the sums
 // are joined; a teacher's entries take eight lanes each, two at a time.
 template <typename T, int kRows, bool TEACHER>
 __global__ void __launch_bounds__(kFinishThreads, TEACHER ? 3 : 5)
@@ -1403,8 +1410,8 @@ struct BwdArgs {
 
 template <typename T>
 static int linear_bwd_t(const BwdArgs& a, const BwdWs& w, cudaStream_t st) {
-  // dz is kept in 16 bits.  In float16 it carries a factor of 2^14 (its values are within [-1, 1]): probabilities down to 2^-38 keep their
-  // 11 bits instead of vanishing below 2^-24; the factor leaves again in the products' float32 results.
+  // dz is kept in 16 bits.  In float16 it carries a factor of 2^14 (its values are within [-1, 1]): probabilities keep 11 bits down to 2^-28
+  // (2^-14 without it) and steps of 2^-38 below (2^-24); the factor leaves again in the products' float32 results.
   const float shift = a.dtype == LANCET_F16 ? 14.f : 0.f;
   const float unit = a.dtype == LANCET_F16 ? 16384.f : 1.f;
   int blocks = (a.rows + 7) / 8;

@@ -53,8 +53,8 @@ class GPTMoE(torch.nn.Module):
                  device="cuda", fabric=None, group=None, seed=0, act="gelu", pipeline=False, fused_head=False, distill_weight=0.5,
                  distill_temperature=1.0):
         """fused_head: the loss is taken from the head's hidden rows without the logits in memory (`linear_cross_entropy`): at
-        8192 tokens and 50257 classes the head needs 1.0 GB beside its operands instead of 1.65 (and no more at larger batches), the
-        step 2 % more time; the default keeps the logits.
+        8192 tokens and 50257 classes the head needs 1.0 GB beside its operands instead of 1.65 (at larger batches the gradient of the logits
+        stays within 1 GiB up to 131072 tokens, 8 KB a token from there on), the step 2 % more time; the default keeps the logits.
         distill_weight, distill_temperature: share and temperature of the distillation loss where `forward` gets a teacher.
         act: activation of every FFN; the reference's GPT-2 uses ReLU (models/benchmark/pytorch/nlp.py:161-165),
         its BERT / ViT GELU (:137-141).  pipeline: the MoE blocks run layer norm, gate projection and residual add

@@ -915,11 +915,12 @@ struct FinishArgs {
 };
 
 // A block finishes kRows packed rows: joins the partial maxima and sums of its rows' column half tiles (in a fixed order), and computes the
-// logits at the rows' targets, or at the entries of their teachers, as float32 dot products.  The tensor cores cut the sums of products short
-// (at a logit of 12 of 1024 products 1e-5 low where they have both signs, 8e-5 where all are positive), which the loss would show where a target (or a teacher's likeliest class) holds most of the
-// probability: its share of the row's sum is replaced by the dot product's.  The other classes keep what was cut: a common offset of 100 in all logits
-// makes the loss 1.4e-4 low at width 1024 (6e-4 at 4096), about what float32 logits scatter by (1.3e-4, 2.8e-4).  That dot product takes a warp and is under way before the sums
-// are joined; a teacher's entries take eight lanes each, two at a time.
+// logits at the rows' targets, or at the entries of their teachers, as float32 dot products.  The tensor cores cut the sums of products short (at
+// a logit of 12 of 1024 products 1e-5 low where they have both signs, 8e-5 where all are positive), which the loss would show where a target (or
+// a teacher's likeliest class) holds most of the probability: its share of the row's sum is replaced by the dot product's.  The other classes
+// keep what was cut: a common offset of 100 in all logits makes the loss 1.4e-4 low at width 1024 (6e-4 at 4096), about what float32 logits
+// scatter by (1.3e-4, 2.8e-4).  That dot product takes a warp and is under way before the sums are joined; a teacher's entries take eight lanes
+// each, two at a time.
 template <typename T, int kRows, bool TEACHER>
 __global__ void __launch_bounds__(kFinishThreads, TEACHER ? 3 : 5)
 finish_rows_kernel(FinishArgs a) {

@@ -919,8 +919,8 @@ struct FinishArgs {
 // a logit of 12 of 1024 products 1e-5 low where they have both signs, 8e-5 where all are positive), which the loss would show where a target (or
 // a teacher's likeliest class) holds most of the probability: its share of the row's sum is replaced by the dot product's.  The other classes
 // keep what was cut: a common offset of 100 in all logits makes the loss 1.4e-4 low at width 1024 (6e-4 at 4096), about what float32 logits
-// scatter by (1.3e-4, 2.8e-4).  That dot product takes a warp and is under way before the sums are joined; a teacher's entries take eight lanes
-// each, two at a time.
+// scatter by (1.3e-4, 2.8e-4).  The dot product of the target takes a warp and is under way before the sums are joined; a teacher's entries take
+// eight lanes each, two at a time.
 template <typename T, int kRows, bool TEACHER>
 __global__ void __launch_bounds__(kFinishThreads, TEACHER ? 3 : 5)
 finish_rows_kernel(FinishArgs a) {
